@@ -16,8 +16,10 @@ SOURCES = ['voxelize.hip', 'rulebook.hip', 'spconv.hip', 'iou3d_nms.hip',
 HEADERS = ['dm_common.h', 'box_geom.h', '../../include/detmatch_hip.h', 'chain_tramp.inc']
 # -ffp-contract=off: fused multiply-adds only where the source says fmaf(), so the
 # CPU oracle (same flag) and the device agree bit for bit on index-deciding math.
+# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 (hipcc -O3 forms them from scalar float code; some of their operand forms
+# have returned wrong results on MI355X).  The host pass warns that it does not know the feature.
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-ffp-contract=off',
-         '-fno-fast-math', '-Wno-unused-result', '-DNDEBUG']
+         '-fno-fast-math', '-Wno-unused-result', '-DNDEBUG', '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 
 
 def _hipcc():
