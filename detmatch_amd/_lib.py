@@ -192,6 +192,8 @@ SIGNATURES = {
     'dm_fill_bytes': (ci, [vp, ci, sz, vp]),
     'dm_bn_fold_batch': (ci, [vp, ci, ci, vp]),
     'dm_multi_add_f32': (ci, [vp, ci, ctypes.c_longlong, ci, vp]),
+    'dm_act8_pack': (ci, [vp, ci, ctypes.c_longlong, ci, ctypes.c_longlong, vp, vp, vp]),
+    'dm_act8_unpack': (ci, [vp, vp, ctypes.c_longlong, ci, vp, ci, vp]),
 }
 
 

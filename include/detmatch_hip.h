@@ -1093,6 +1093,19 @@ int dm_fill_bytes(void *dst, int byte_value, size_t nbytes, dm_stream_t stream);
 int dm_bn_fold_batch(const void *table_dev, int n_rows, int max_channels, dm_stream_t stream);
 int dm_multi_add_f32(const void *table_dev, int n_rows, long long max_n, int assign, dm_stream_t stream);
 
+/* ------------------------------------------------------------------------ */
+/* Activations kept in 8 bits between the forward and the backward pass.  dtype: 0 fp32, 1 bf16, 2 fp16.
+ * A row of `width` channels becomes groups = ceil(width / 32) groups; a group has e4m3 codes (1 sign, 4 exponent, 3 mantissa
+ * bits, no infinities) and one exponent byte e + 127: value = code * 2^e, e = the least exponent >= -127 with
+ * max |x| <= 448 * 2^e over the finite values of the group (0 for a group of zeros), codes rounded to nearest even; inf and nan
+ * become nan.
+ *   dm_act8_pack     x (rows, width), row stride ld elements -> codes (rows, 32 * groups; 0 behind the width), exps (rows, groups)
+ *   dm_act8_unpack   the values, in `dtype` (saturating at its largest finite value), dense (rows, width) */
+int dm_act8_pack(const void *x, int dtype, long long rows, int width, long long ld, uint8_t *codes, uint8_t *exps,
+                 dm_stream_t stream);
+int dm_act8_unpack(const uint8_t *codes, const uint8_t *exps, long long rows, int width, void *out, int dtype,
+                   dm_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
