@@ -194,6 +194,9 @@ SIGNATURES = {
     'dm_multi_add_f32': (ci, [vp, ci, ctypes.c_longlong, ci, vp]),
     'dm_act8_pack': (ci, [vp, ci, ctypes.c_longlong, ci, ctypes.c_longlong, vp, vp, vp]),
     'dm_act8_unpack': (ci, [vp, vp, ctypes.c_longlong, ci, vp, ci, vp]),
+    'dm_act8_gemm_workspace_bytes': (sz, [ci, ci, ci, ci, ci]),
+    'dm_act8_gemm': (ci, [ci, ci, vp, ctypes.c_longlong, vp, ctypes.c_longlong, vp, vp, ci, ci, ci, ci, vp, vp, vp, vp, sz, vp]),
+    'dm_act8_mask_rows': (ci, [vp, ci, ctypes.c_longlong, ci, ctypes.c_longlong, vp, vp, ci, vp]),
 }
 
 

@@ -7,8 +7,14 @@ off by at most 2^-4 of a value (half a step), or 2^-10 of the group's scale belo
     kept = pack(x)              Act8: codes + exponents of x (..., C)
     x8 = unpack(kept)           the values that the codes stand for, in x's type
 
-`pack` / `unpack` are plain functions (no gradient)."""
+    y = linear(x, w, b, relu)   [relu](x w^T + b), with gradients; what waits for the backward pass is pack(x), one bit per
+                                output behind a ReLU, and w
+
+`pack` / `unpack` are plain functions (no gradient).  The forward pass and the input gradient of `linear` see x and w as they are;
+only the weight gradient sees unpack(pack(x))."""
 import torch
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -95,3 +101,107 @@ def unpack(kept, dtype=None):
         _lib.check(_lib.lib().dm_act8_unpack(_lib.ptr(kept.codes), _lib.ptr(kept.exps), kept.codes.shape[0], kept.shape[-1],
                                              _lib.ptr(out), code, _lib.stream()), 'dm_act8_unpack')
     return out
+
+
+# ---- fully connected layers ----------------------------------------------------------------------------------------------
+_MAX = (1 << 31) - 1024                      # rows and channels are 32-bit numbers in the kernels
+
+
+def _operand(r, dtype_code):
+    """(tensor, pitch) of rows that dm_act8_gemm reads: r itself, or for 16-bit rows that 16-byte reads do not fit, a copy
+    with a pitch of 8 elements and zeros behind the width."""
+    pitch = row_stride(r)
+    if dtype_code == 0 or (r.shape[1] % 8 == 0 and pitch % 8 == 0 and r.data_ptr() % 16 == 0):
+        return r, pitch
+    return _masked(r, None, dtype_code)
+
+
+def _masked(r, bits, dtype_code):
+    rows, width = r.shape
+    pitch = (width + 7) // 8 * 8
+    out = torch.empty((rows, pitch), dtype=r.dtype, device=r.device)
+    _lib.check(_lib.lib().dm_act8_mask_rows(_lib.ptr(r), dtype_code, rows, width, row_stride(r), _lib.ptr(bits), _lib.ptr(out),
+                                            pitch, _lib.stream()), 'dm_act8_mask_rows')
+    return out, pitch
+
+
+def _gemm(form, code, a, b, exps, bias, relu, m, n, k, out, bits=None, rowsum=None):
+    """a, b: (tensor, pitch)"""
+    L = _lib.lib()
+    need = int(L.dm_act8_gemm_workspace_bytes(form, code, m, n, k))
+    # (a buffer of its own for every call: two streams, or two captured graphs, never share one)
+    ws = torch.empty(need, dtype=torch.uint8, device=out.device) if need else None
+    _lib.check(L.dm_act8_gemm(form, code, _lib.ptr(a[0]), a[1], _lib.ptr(b[0]), b[1], _lib.ptr(exps), _lib.ptr(bias), int(relu), m, n,
+                              k, _lib.ptr(out), _lib.ptr(bits), _lib.ptr(rowsum), _lib.ptr(ws), need, _lib.stream()), 'dm_act8_gemm')
+    return out
+
+
+class _Linear8(Function):
+
+    @staticmethod
+    def forward(ctx, x, w, b, relu):
+        code = DTYPES[x.dtype]
+        m, k = x.shape
+        n = w.shape[0]
+        needs = ctx.needs_input_grad
+        with torch.cuda.device(x.device):
+            y = torch.empty((m, n), dtype=x.dtype, device=x.device)
+            bits = torch.empty((m, (n + 31) // 32), dtype=torch.int32, device=x.device) if relu and any(needs[:3]) else None
+            kept = pack(x) if needs[1] else None
+            if m:
+                _gemm(0, code, _operand(rows_view(x.detach()), code), _operand(rows_view(w.detach()), code), None,
+                      None if b is None else b.detach().contiguous(), relu, m, n, k, y, bits)
+        ctx.save_for_backward(w if needs[0] else None, kept.codes if kept else None, kept.exps if kept else None, bits)
+        ctx.sizes = (m, n, k)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        w, codes, exps, bits = ctx.saved_tensors
+        m, n, k = ctx.sizes
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        code = DTYPES[gy.dtype]
+        gx = gw = gb = None
+        with torch.cuda.device(gy.device):
+            if m == 0:
+                return (gy.new_zeros((0, k)) if need_x else None, gy.new_zeros((n, k)) if need_w else None,
+                        gy.new_zeros(n) if need_b else None, None)
+            g = rows_view(gy)
+            g = _operand(g, code) if bits is None else _masked(g, bits, code)
+            if need_x:
+                gx = _gemm(1, code, g, _operand(rows_view(w.detach()), code), None, None, False, m, k, n,
+                           torch.empty((m, k), dtype=gy.dtype, device=gy.device))
+            if need_w or need_b:
+                gb = torch.empty(n, dtype=gy.dtype, device=gy.device) if need_b else None
+                if need_w:
+                    gw = torch.empty((n, k), dtype=gy.dtype, device=gy.device)
+                    _gemm(2, code, g, (codes, codes.shape[1]), exps, None, False, n, k, m, gw, rowsum=gb)
+                else:                         # a bias alone: its sums ride on a product with one group of zeros
+                    zero = torch.zeros((m, GROUP + 1), dtype=torch.uint8, device=gy.device)
+                    _gemm(2, code, g, (zero[:, :GROUP].contiguous(), GROUP), zero[:, GROUP:].contiguous(), None, False, n, GROUP, m,
+                          torch.empty((n, GROUP), dtype=gy.dtype, device=gy.device), rowsum=gb)
+        return gx, gw, gb, None
+
+
+def linear(x, w, b=None, relu=False):
+    """[relu](x w^T + b) for x (..., in), w (out, in), b (out) of one type (float32, bfloat16 or float16), on csrc/act8_gemm.hip.
+
+    Kept for the backward pass: pack(x) where w needs a gradient, one bit per output where there is a ReLU, w where x needs a
+    gradient.  gw = g^T unpack(pack(x)), gx = g w, gb = sum of g over rows, g = the gradient behind the ReLU (0 where its output
+    is 0).  x may be overwritten after the call.  Differentiable once."""
+    if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1]:
+        raise ValueError('x (..., in) and w (out, in) are wanted, got %s and %s' % (tuple(x.shape), tuple(w.shape)))
+    if b is not None and tuple(b.shape) != (w.shape[0],):
+        raise ValueError('b has shape %s, w has %d rows' % (tuple(b.shape), w.shape[0]))
+    if w.shape[0] < 1 or w.shape[1] < 1:
+        raise ValueError('w %s has no elements' % (tuple(w.shape),))
+    _dtype_code(x, 'x')
+    for t, name in ((w, 'w'), (b, 'b')):
+        if t is not None and t.dtype != x.dtype:
+            raise TypeError('%s is %s, x is %s: one type is wanted' % (name, t.dtype, x.dtype))
+    _device_of(x, w, b)
+    x2 = x.reshape(-1, x.shape[-1])
+    if max(x2.shape[0], w.shape[0], w.shape[1]) > _MAX:
+        raise ValueError('sizes up to %d are wanted, got x %s, w %s' % (_MAX, tuple(x.shape), tuple(w.shape)))
+    return _Linear8.apply(x2, w, b, bool(relu)).view(*x.shape[:-1], w.shape[0])

@@ -1,0 +1,660 @@
+// Matrix products of an FC layer whose weight gradient reads the 8-bit copy of its input (act8_codec.h).
+//   form 0   C[M][N] = A[M][K] . B[N][K]^T (+ bias, ReLU, sign bits)   forward            y  = x w^T + b
+//   form 1   C[M][N] = A[M][K] . B[K][N]                               input gradient     gx = gy w
+//   form 2   C[M][N] = A[K][M]^T . deq(B)[K][N] (+ row sums)           weight gradient    gw = gy^T x8, gb = sum of gy
+// All on the 16-bit matrix instructions (v_mfma_f32_32x32x16), accumulated in fp32.  deq(code) is exact in bf16, so form 2 loses nothing
+// there.  fp32 operands are cut into three bf16 pieces (8 + 8 + 8 bits: exact for finite values) while they are staged; a product
+// of two such operands takes the 6 of the 9 piece products that matter in fp32, a product with codes takes 3.
+//
+// A wave owns FM x FN blocks of 32 x 32; the matrix instruction gets its operands swapped (rows of its result = columns of C), so that a
+// lane ends with 4 neighbouring elements of a row of C.  Few output tiles and a long contraction: the contraction is split over
+// workgroups, partial sums go to a workspace and are added in split order by a second kernel (no atomics: the result is a
+// function of the shapes and values alone).
+#include "act8_codec.h"
+
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+__device__ __attribute__((aligned(16))) const uint32_t a8_zeros[4] = {0, 0, 0, 0};   // source of what lies outside of an operand
+
+struct A8Args {
+  const void *A, *B, *bias;
+  const uint8_t *exps;        // form 2: exponents of B's codes, groups per row = ldb / 32
+  void *C;
+  float *part;                // [splits][M][N] when splits > 1, and behind it [splits][M] row sums
+  uint32_t *bits;             // sign bits of C > 0, (M, ceil(N / 32))
+  void *rowsum;               // form 2: sum over the contraction of A's columns (M)
+  int M, N, K;
+  long long lda, ldb;
+  int relu, splits, steps_per_split, tiles_m, tiles_n, per_xcd, vec_a, vec_b, vec_c;
+};
+
+// ---- where a 16-byte piece of a staged tile lies in LDS ----------------------------------------------------------------
+// contraction-contiguous tile [rows][BK]: a fragment read takes the same piece of 16 rows at once; the piece index is xored with bits
+// of the row, so that those 16 reads fall on all 64 banks.
+template <int BK>
+__device__ __forceinline__ int kc_swizzle(int row) {
+  return BK == 64 ? (row >> 1) & 7 : (row >> 2) & 3;
+}
+// contraction along the rows [BK][cols], 128-column (256-byte) lines or wider: a transposing read takes 64 bytes of 4 rows at once, a
+// staging store the pieces 2 c + j of 2 rows
+__device__ __forceinline__ int kr_swizzle(int k) { return ((k & 3) << 2) | (k & 1); }
+
+// fragment of 32 rows x 16 of the contraction from a contraction-contiguous tile: lane -> row lane & 31, 8 elements from (lane >> 5) * 8
+template <int BK>
+__device__ __forceinline__ s16x8 frag_kc(const uint16_t *S, int row0, int kk, int lane) {
+  const int row = row0 + (lane & 31), c = (kk * 2 + (lane >> 5)) ^ kc_swizzle<BK>(row);
+  return *(const s16x8 *)(S + row * BK + c * 8);
+}
+
+// the same fragment from a tile whose rows run along the contraction: two transposing reads; lane i of a group of 16 reads 4 columns
+// of row i / 4 and receives 4 rows of column i
+template <int COLS>
+__device__ __forceinline__ s16x8 frag_kr(const uint16_t *S, int col0, int kk, int lane) {
+  const int i = lane & 15, col = col0 + ((lane >> 4) & 1) * 16 + (i & 3) * 4;
+  const int k = kk * 16 + (lane >> 5) * 8 + (i >> 2);
+  // (k and k + 4 have the same swizzle)
+  const uint16_t *p = S + k * COLS + (((col >> 3) ^ kr_swizzle(k)) * 8 + (col & 7));
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)p);
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p + 4 * COLS));
+  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+template <int T>
+__device__ __forceinline__ f32x16 mfma16(s16x8 a, s16x8 b, f32x16 c) {
+  if constexpr (T == ACT8_F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// 4 codes * 2^e -> 4 values of the 16-bit type (the exponent byte is the exponent field of the instruction's scale)
+template <int T>
+__device__ __forceinline__ uint2 deq4(uint32_t u, uint32_t eb) {
+  const float scale = __uint_as_float(eb << 23);
+  if constexpr (T == ACT8_F16) {
+    if (eb >= 127 + 8) {                        // 256 * 2^8 is the one value that fp16 does not have: saturate
+      float v[4];
+      act8_decode4(u, (int)eb - 127, v);
+      union { uint2 w; _Float16 h[4]; } r;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) r.h[k] = (_Float16)(v[k] != v[k] ? v[k] : fminf(fmaxf(v[k], -65504.f), 65504.f));
+      return r.w;
+    }
+    const f16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)u, scale, false);
+    const f16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)u, scale, true);
+    return make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
+  } else {
+    const bf16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)u, scale, false);
+    const bf16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)u, scale, true);
+    return make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
+  }
+}
+
+// three bf16 pieces of two fp32 values each: the leading 8 bits, the next 8, the last 8 (truncated, so that nothing overflows)
+__device__ __forceinline__ void split3(float a, float b, uint32_t *p) {
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    const uint32_t ua = __float_as_uint(a) & 0xffff0000u, ub = __float_as_uint(b) & 0xffff0000u;
+    p[k] = (ua >> 16) | ub;
+    a -= __uint_as_float(ua), b -= __uint_as_float(ub);
+  }
+}
+
+// ---- tile staging ------------------------------------------------------------------------------------------------------
+typedef const __attribute__((address_space(1))) void *gptr_t;
+typedef __attribute__((address_space(3))) void *lptr_t;
+
+// 16-bit operand, 16-byte pieces straight from memory into LDS.  A wave's 64 pieces land side by side; the swizzle is in the
+// address that each lane reads.  Rows behind the operand repeat its last one (their results are not stored); the contraction
+// behind its end is 0.  (Rows are readable, and 0 along the contraction, up to the next multiple of 8 elements: the entry's contract.)
+template <int ROWS, int BK, int THREADS>
+__device__ __forceinline__ void stage_kc(uint16_t *S, const uint16_t *P, long long ld, int rows, int k0, int k_hi, int tid) {
+#pragma unroll
+  for (int h = 0; h < ROWS * BK / 8 / THREADS; ++h) {
+    const int i = tid + THREADS * h, row = i / (BK / 8), c = (i % (BK / 8)) ^ kc_swizzle<BK>(row), k = k0 + 8 * c;
+    const uint16_t *src = k < k_hi ? P + (long long)min(row, rows - 1) * ld + k : (const uint16_t *)a8_zeros;
+    __builtin_amdgcn_global_load_lds((gptr_t)src, (lptr_t)(S + (size_t)(i - (tid & 63)) * 8), 16, 0, 0);
+  }
+}
+
+template <int COLS, int BK, int THREADS>
+__device__ __forceinline__ void stage_kr(uint16_t *S, const uint16_t *P, long long ld, int cols, int k0, int k_hi, int tid) {
+#pragma unroll
+  for (int h = 0; h < COLS * BK / 8 / THREADS; ++h) {
+    const int i = tid + THREADS * h, r = i / (COLS / 8), c = (i % (COLS / 8)) ^ kr_swizzle(r), k = k0 + r;
+    const uint16_t *src = k < k_hi ? P + (long long)k * ld + min(8 * c, ((cols + 7) & ~7) - 8) : (const uint16_t *)a8_zeros;
+    __builtin_amdgcn_global_load_lds((gptr_t)src, (lptr_t)(S + (size_t)(i - (tid & 63)) * 8), 16, 0, 0);
+  }
+}
+
+// 8-bit operand: 16 codes of a row at a time through registers
+template <int COLS, int BK, int THREADS>
+struct CodeRegs {
+  static constexpr int H = COLS * BK / 16 / THREADS;
+  uint4 u[H];
+  uint32_t e[H];
+};
+
+template <int COLS, int BK, int THREADS>
+__device__ __forceinline__ void fetch_codes(CodeRegs<COLS, BK, THREADS> &t, const uint8_t *P, const uint8_t *E, long long ld, int n0,
+                                            int k0, int k_hi, int tid) {
+#pragma unroll
+  for (int h = 0; h < CodeRegs<COLS, BK, THREADS>::H; ++h) {
+    const int i = tid + THREADS * h, k = k0 + i / (COLS / 16), c = n0 + 16 * (i % (COLS / 16));
+    t.u[h] = make_uint4(0, 0, 0, 0), t.e[h] = 127;
+    if (k < k_hi && c < ld) {
+      t.u[h] = *(const uint4 *)(P + (long long)k * ld + c);
+      t.e[h] = E[(long long)k * (ld / 32) + c / 32];
+    }
+  }
+}
+
+template <int T, int COLS, int BK, int THREADS>
+__device__ __forceinline__ void store_codes(const CodeRegs<COLS, BK, THREADS> &t, uint16_t *S, int tid) {
+#pragma unroll
+  for (int h = 0; h < CodeRegs<COLS, BK, THREADS>::H; ++h) {
+    const int i = tid + THREADS * h, r = i / (COLS / 16), c = 2 * (i % (COLS / 16)), z = kr_swizzle(r);
+    const uint2 a = deq4<T>(t.u[h].x, t.e[h]), b = deq4<T>(t.u[h].y, t.e[h]), d = deq4<T>(t.u[h].z, t.e[h]), f = deq4<T>(t.u[h].w, t.e[h]);
+    *(uint4 *)(S + r * COLS + ((c ^ z) * 8)) = make_uint4(a.x, a.y, b.x, b.y);
+    *(uint4 *)(S + r * COLS + (((c + 1) ^ z) * 8)) = make_uint4(d.x, d.y, f.x, f.y);
+  }
+}
+
+// fp32 operand: 8 elements at a time through registers, three planes in LDS
+template <int ROWS, int BK, int THREADS>
+struct F32Regs {
+  static constexpr int H = ROWS * BK / 8 / THREADS;
+  float v[H][8];
+};
+
+template <bool ALONG_K, int ROWS, int BK, int THREADS>
+__device__ __forceinline__ void fetch_f32(F32Regs<ROWS, BK, THREADS> &t, const float *P, long long ld, int row0, int rows, int k0, int k_hi,
+                                          int tid, bool vec) {
+#pragma unroll
+  for (int h = 0; h < F32Regs<ROWS, BK, THREADS>::H; ++h) {
+    const int i = tid + THREADS * h;
+    int n;                                    // elements of this piece that exist
+    long long at;
+    if (!ALONG_K) {
+      const int row = row0 + i / (BK / 8), k = k0 + 8 * (i % (BK / 8));
+      n = row < rows ? k_hi - k : 0;
+      at = (long long)row * ld + k;
+    } else {
+      const int k = k0 + i / (ROWS / 8), row = row0 + 8 * (i % (ROWS / 8));
+      n = k < k_hi ? rows - row : 0;
+      at = (long long)k * ld + row;
+    }
+    act8_load8<ACT8_F32>(P, (size_t)at, n, vec, t.v[h]);
+  }
+}
+
+template <bool ALONG_K, int ROWS, int BK, int THREADS>
+__device__ __forceinline__ void store_f32(const F32Regs<ROWS, BK, THREADS> &t, uint16_t *S, int tid) {
+#pragma unroll
+  for (int h = 0; h < F32Regs<ROWS, BK, THREADS>::H; ++h) {
+    const int i = tid + THREADS * h;
+    int at;
+    if (!ALONG_K) {
+      const int r = i / (BK / 8);
+      at = r * BK + ((i % (BK / 8)) ^ kc_swizzle<BK>(r)) * 8;
+    } else {
+      const int r = i / (ROWS / 8);
+      at = r * ROWS + ((i % (ROWS / 8)) ^ kr_swizzle(r)) * 8;
+    }
+    uint32_t p[4][3];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) split3(t.v[h][2 * k], t.v[h][2 * k + 1], p[k]);
+#pragma unroll
+    for (int q = 0; q < 3; ++q) *(uint4 *)(S + q * ROWS * BK + at) = make_uint4(p[0][q], p[1][q], p[2][q], p[3][q]);
+  }
+}
+
+// ---- tile order and epilogue -------------------------------------------------------------------------------------------
+struct Tile {
+  int m, n, split;
+};
+
+// workgroup ids go round-robin over the 8 XCDs (each with its own L2): an XCD gets consecutive logical tiles, and those go
+// down 8 tile rows at a time, so that the tiles in flight on one XCD share rows of A and columns of B
+__device__ __forceinline__ bool tile_of(const A8Args &a, Tile *t) {
+  const int logical = (int)(blockIdx.x % 8) * a.per_xcd + (int)(blockIdx.x / 8), tiles = a.tiles_m * a.tiles_n;
+  if (logical >= tiles * a.splits) return false;
+  t->split = logical / tiles;
+  const int i = logical - t->split * tiles, band = i / (8 * a.tiles_n), m_lo = band * 8, high = min(8, a.tiles_m - m_lo);
+  const int j = i - band * 8 * a.tiles_n;
+  t->m = m_lo + j % high, t->n = j / high;
+  return true;
+}
+
+// 4 neighbouring elements of row m from n on
+template <int T>
+__device__ __forceinline__ void finish4(const A8Args &a, int m, int n, float *v) {
+  if (a.bias) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (n + k < a.N) v[k] += act8_get<T>(a.bias, n + k);
+  }
+}
+
+template <int T>
+__device__ __forceinline__ void put4(const A8Args &a, int m, int n, const float *v) {
+  const size_t at = (size_t)m * a.N + n;
+  if (a.vec_c && n + 3 < a.N) {
+    if constexpr (T == ACT8_F32) *(float4 *)((float *)a.C + at) = make_float4(v[0], v[1], v[2], v[3]);
+    else {
+      union { uint2 w; uint16_t h[4]; } u;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) act8_put<T>(u.h, k, v[k]);
+      *(uint2 *)((uint16_t *)a.C + at) = u.w;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (n + k < a.N) act8_put<T>(a.C, at + k, v[k]);
+  }
+}
+
+// one 32 x 32 block: lane -> row m0 + (lane & 31), columns n0 + 8 q + 4 (lane >> 5) + 0..3 for q = 0..3
+template <int T>
+__device__ __forceinline__ void store_block(const A8Args &a, const Tile &t, const f32x16 &acc, int m0, int n0, int lane) {
+  const int m = m0 + (lane & 31);
+  uint32_t word = 0;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int n = n0 + 8 * q + 4 * (lane >> 5);
+    float v[4] = {acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+    if (a.splits > 1) {
+      float *p = a.part + ((size_t)t.split * a.M + m) * a.N + n;
+      if (m < a.M) {
+        if (a.N % 4 == 0 && n + 3 < a.N) *(float4 *)p = make_float4(v[0], v[1], v[2], v[3]);
+        else
+          for (int k = 0; k < 4; ++k)
+            if (n + k < a.N) p[k] = v[k];
+      }
+      continue;
+    }
+    finish4<T>(a, m, n, v);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (v[k] > 0.f) word |= 1u << (8 * q + 4 * (lane >> 5) + k);
+      if (a.relu) v[k] = v[k] < 0.f ? 0.f : v[k];            // (a nan stays one)
+    }
+    if (m < a.M) put4<T>(a, m, n, v);
+  }
+  if (a.bits && a.splits == 1) {
+    word |= __shfl_xor(word, 32);
+    if (lane < 32 && m < a.M && n0 < a.N) a.bits[(size_t)m * ((a.N + 31) / 32) + n0 / 32] = word;
+  }
+}
+
+// ---- the 16-bit product --------------------------------------------------------------------------------------------------
+template <int T, int FORM, int WM, int WN, int FM, int FN>
+__global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 ? 2 : 1) void a8_gemm16_kernel(A8Args a) {
+  constexpr int BM = WM * FM * 32, BN = WN * FN * 32, BK = 64, THREADS = 64 * WM * WN;
+  extern __shared__ __attribute__((aligned(16))) uint16_t a8_lds[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / WN, wn = wave % WN;
+  Tile t;
+  if (!tile_of(a, &t)) return;
+  const int m0 = t.m * BM, n0 = t.n * BN;
+  const int s_lo = t.split * a.steps_per_split, s_hi = min((a.K + BK - 1) / BK, s_lo + a.steps_per_split);
+  const uint16_t *A = (const uint16_t *)a.A + (FORM == 2 ? (long long)m0 : (long long)m0 * a.lda);
+  const uint16_t *B = (const uint16_t *)a.B + (FORM == 1 ? (long long)n0 : (long long)n0 * a.ldb);      // (form 2: unused)
+  const bool sums = FORM == 2 && a.rowsum && t.n == 0 && wn == 0;
+  f32x16 acc[FM][FN], sum[FORM == 2 ? FM : 1];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+#pragma unroll
+  for (int i = 0; i < (FORM == 2 ? FM : 1); ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sum[i][r] = 0.f;
+  const short one = T == ACT8_F16 ? 0x3c00 : 0x3f80;
+  const s16x8 ones = {one, one, one, one, one, one, one, one};
+  CodeRegs<BN, BK, THREADS> codes;
+
+  auto stage = [&](int s, int buf) {
+    const int k0 = s * BK;
+    if constexpr (FORM == 2) {
+      stage_kr<BM, BK, THREADS>((a8_lds + buf * BM * BK), A, a.lda, a.M - m0, k0, a.K, tid);
+      fetch_codes<BN, BK, THREADS>(codes, (const uint8_t *)a.B, a.exps, a.ldb, n0, k0, a.K, tid);
+    } else {
+      stage_kc<BM, BK, THREADS>((a8_lds + buf * BM * BK), A, a.lda, a.M - m0, k0, a.K, tid);
+      if constexpr (FORM == 0) stage_kc<BN, BK, THREADS>((a8_lds + 2 * BM * BK + buf * BN * BK), B, a.ldb, a.N - n0, k0, a.K, tid);
+      else stage_kr<BN, BK, THREADS>((a8_lds + 2 * BM * BK + buf * BN * BK), B, a.ldb, a.N - n0, k0, a.K, tid);
+    }
+  };
+
+  if (s_lo < s_hi) {
+    stage(s_lo, 0);
+    if constexpr (FORM == 2) store_codes<T, BN, BK, THREADS>(codes, a8_lds + 2 * BM * BK, tid);
+  }
+  for (int s = s_lo; s < s_hi; ++s) {
+    const int buf = (s - s_lo) & 1;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // this step's tiles have landed ...
+    __syncthreads();                                      // ... for all waves, and nobody reads the other pair any more
+    if (s + 1 < s_hi) stage(s + 1, buf ^ 1);
+#pragma unroll
+    for (int kk = 0; kk < BK / 16; ++kk) {
+      s16x8 fa[FM], fb[FN];
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        if constexpr (FORM == 2) fa[i] = frag_kr<BM>((a8_lds + buf * BM * BK), (wm * FM + i) * 32, kk, lane);
+        else fa[i] = frag_kc<BK>((a8_lds + buf * BM * BK), (wm * FM + i) * 32, kk, lane);
+      }
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        if constexpr (FORM == 0) fb[j] = frag_kc<BK>((a8_lds + 2 * BM * BK + buf * BN * BK), (wn * FN + j) * 32, kk, lane);
+        else fb[j] = frag_kr<BN>((a8_lds + 2 * BM * BK + buf * BN * BK), (wn * FN + j) * 32, kk, lane);
+      }
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = mfma16<T>(fb[j], fa[i], acc[i][j]);
+      if constexpr (FORM == 2) {
+        if (sums) {
+#pragma unroll
+          for (int i = 0; i < FM; ++i) sum[i] = mfma16<T>(ones, fa[i], sum[i]);
+        }
+      }
+    }
+    if constexpr (FORM == 2) {
+      if (s + 1 < s_hi) store_codes<T, BN, BK, THREADS>(codes, a8_lds + 2 * BM * BK + (buf ^ 1) * BN * BK, tid);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) store_block<T>(a, t, acc[i][j], m0 + (wm * FM + i) * 32, n0 + (wn * FN + j) * 32, lane);
+  if constexpr (FORM == 2) {
+    if (sums && lane < 32) {
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        const int m = m0 + (wm * FM + i) * 32 + lane;
+        if (m >= a.M) continue;
+        if (a.splits > 1) a.part[(size_t)a.splits * a.M * a.N + (size_t)t.split * a.M + m] = sum[i][0];
+        else act8_put<T>(a.rowsum, m, sum[i][0]);
+      }
+    }
+  }
+}
+
+// ---- the fp32 product ----------------------------------------------------------------------------------------------------
+// 128 x 128 tile, 4 waves of 64 x 64, 32 of the contraction at a time; the next step's operands are in registers while this
+// one's planes are multiplied.
+template <int FORM>
+__global__ __launch_bounds__(256) void a8_gemm32_kernel(A8Args a) {
+  constexpr int BM = 128, BN = 128, BK = 32, THREADS = 256, FM = 2, FN = 2, PB = FORM == 2 ? 1 : 3;
+  extern __shared__ __attribute__((aligned(16))) uint16_t a8_lds[];
+  uint16_t *As = a8_lds, *Bs = a8_lds + 3 * BM * BK;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
+  Tile t;
+  if (!tile_of(a, &t)) return;
+  const int m0 = t.m * BM, n0 = t.n * BN;
+  const int s_lo = t.split * a.steps_per_split, s_hi = min((a.K + BK - 1) / BK, s_lo + a.steps_per_split);
+  const bool sums = FORM == 2 && a.rowsum && t.n == 0 && wn == 0;
+  f32x16 acc[FM][FN], sum[FM];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      sum[i][r] = 0.f;
+#pragma unroll
+      for (int j = 0; j < FN; ++j) acc[i][j][r] = 0.f;
+    }
+  const short one = 0x3f80;
+  const s16x8 ones = {one, one, one, one, one, one, one, one};
+  F32Regs<BM, BK, THREADS> ra;
+  F32Regs<BN, BK, THREADS> rb;
+  CodeRegs<BN, BK, THREADS> codes;
+
+  auto fetch = [&](int s) {
+    fetch_f32<FORM == 2, BM, BK, THREADS>(ra, (const float *)a.A, a.lda, m0, a.M, s * BK, a.K, tid, a.vec_a != 0);
+    if constexpr (FORM == 2) fetch_codes<BN, BK, THREADS>(codes, (const uint8_t *)a.B, a.exps, a.ldb, n0, s * BK, a.K, tid);
+    else fetch_f32<FORM == 1, BN, BK, THREADS>(rb, (const float *)a.B, a.ldb, n0, a.N, s * BK, a.K, tid, a.vec_b != 0);
+  };
+
+  if (s_lo < s_hi) fetch(s_lo);
+  for (int s = s_lo; s < s_hi; ++s) {
+    __syncthreads();                                      // the previous step's fragments have been read
+    store_f32<FORM == 2, BM, BK, THREADS>(ra, As, tid);
+    if constexpr (FORM == 2) store_codes<ACT8_BF16, BN, BK, THREADS>(codes, Bs, tid);
+    else store_f32<FORM == 1, BN, BK, THREADS>(rb, Bs, tid);
+    __syncthreads();
+    if (s + 1 < s_hi) fetch(s + 1);
+#pragma unroll
+    for (int kk = 0; kk < BK / 16; ++kk) {
+      s16x8 fa[3][FM], fb[PB][FN];
+#pragma unroll
+      for (int q = 0; q < 3; ++q)
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+          if constexpr (FORM == 2) fa[q][i] = frag_kr<BM>(As + q * BM * BK, (wm * FM + i) * 32, kk, lane);
+          else fa[q][i] = frag_kc<BK>(As + q * BM * BK, (wm * FM + i) * 32, kk, lane);
+        }
+#pragma unroll
+      for (int q = 0; q < PB; ++q)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+          if constexpr (FORM == 0) fb[q][j] = frag_kc<BK>(Bs + q * BN * BK, (wn * FN + j) * 32, kk, lane);
+          else fb[q][j] = frag_kr<BN>(Bs + q * BN * BK, (wn * FN + j) * 32, kk, lane);
+        }
+      // smallest products first
+#pragma unroll
+      for (int o = 2; o >= 0; --o)
+#pragma unroll
+        for (int q = 0; q < PB; ++q) {
+          if (o - q < 0) continue;
+#pragma unroll
+          for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[i][j] = mfma16<ACT8_BF16>(fb[q][j], fa[o - q][i], acc[i][j]);
+        }
+      if constexpr (FORM == 2) {
+        if (sums) {
+#pragma unroll
+          for (int q = 2; q >= 0; --q)
+#pragma unroll
+            for (int i = 0; i < FM; ++i) sum[i] = mfma16<ACT8_BF16>(ones, fa[q][i], sum[i]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) store_block<ACT8_F32>(a, t, acc[i][j], m0 + (wm * FM + i) * 32, n0 + (wn * FN + j) * 32, lane);
+  if constexpr (FORM == 2) {
+    if (sums && lane < 32) {
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        const int m = m0 + (wm * FM + i) * 32 + lane;
+        if (m >= a.M) continue;
+        if (a.splits > 1) a.part[(size_t)a.splits * a.M * a.N + (size_t)t.split * a.M + m] = sum[i][0];
+        else ((float *)a.rowsum)[m] = sum[i][0];
+      }
+    }
+  }
+}
+
+// ---- partial sums, in split order ---------------------------------------------------------------------------------------
+// a thread has 4 neighbouring columns; the last workgroups take the row sums
+template <int T>
+__global__ __launch_bounds__(256) void a8_reduce_kernel(A8Args a, int col4, unsigned main_blocks) {
+  if (blockIdx.x >= main_blocks) {
+    const long long m = (long long)(blockIdx.x - main_blocks) * 256 + threadIdx.x;
+    if (m >= a.M) return;
+    const float *p = a.part + (size_t)a.splits * a.M * a.N + m;
+    float v = 0.f;
+    for (int s = 0; s < a.splits; ++s) v += p[(size_t)s * a.M];
+    act8_put<T>(a.rowsum, m, v);
+    return;
+  }
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const int m = (int)(i / col4), n = 4 * (int)(i % col4);     // col4: a multiple of 8 (a word of sign bits is 8 threads)
+  if (m >= a.M) return;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  const float *p = a.part + (size_t)m * a.N + n;
+  for (int s = 0; s < a.splits; ++s, p += (size_t)a.M * a.N) {
+    if (a.N % 4 == 0 && n + 3 < a.N) {
+      const float4 w = *(const float4 *)p;
+      v[0] += w.x, v[1] += w.y, v[2] += w.z, v[3] += w.w;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (n + k < a.N) v[k] += p[k];
+    }
+  }
+  finish4<T>(a, m, n, v);
+  uint32_t word = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (v[k] > 0.f) word |= 1u << ((n & 31) + k);
+    if (a.relu) v[k] = v[k] < 0.f ? 0.f : v[k];
+  }
+  put4<T>(a, m, n, v);
+  if (a.bits) {
+    word |= __shfl_xor(word, 1), word |= __shfl_xor(word, 2), word |= __shfl_xor(word, 4);
+    if ((n & 31) == 0 && n < a.N) a.bits[(size_t)m * ((a.N + 31) / 32) + n / 32] = word;
+  }
+}
+
+// ---- a gradient behind a ReLU / rows moved to a 16-byte pitch --------------------------------------------------------------
+// out (rows, ldo) = bits ? (bit set ? x : 0) : x, 0 behind the width; a thread has 8 elements
+template <int T>
+__global__ __launch_bounds__(256) void a8_mask_kernel(const void *__restrict__ x, long long rows, int width, long long ld, int vec,
+                                                      const uint32_t *__restrict__ bits, void *__restrict__ out, int ldo) {
+  const int chunks = ldo / 8;
+  const long long total = rows * chunks;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+    const long long r = i / chunks;
+    const int c = 8 * (int)(i % chunks);
+    float v[8];
+    act8_load8<T>(x, (size_t)r * ld + c, width - c, vec != 0, v);
+    if (bits && c < width) {
+      const uint32_t w = bits[r * ((width + 31) / 32) + c / 32] >> (c & 31);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = (w >> k) & 1 ? v[k] : 0.f;
+    }
+    act8_store8<T>(out, (size_t)r * ldo + c, 8, true, v);
+  }
+}
+
+struct Plan {
+  int bm, bn, bk, tiles_m, tiles_n, splits, steps_per_split;
+};
+
+Plan a8_plan(int dtype, int M, int N, int K) {
+  Plan p;
+  p.bm = p.bn = 128;
+  p.bk = dtype == ACT8_F32 ? 32 : 64;
+  p.tiles_m = dm_ceil_div(M, p.bm), p.tiles_n = dm_ceil_div(N, p.bn);
+  const long long tiles = (long long)p.tiles_m * p.tiles_n;
+  const int steps = dm_ceil_div(K, p.bk);
+  long long want = tiles >= 256 ? 1 : (512 + tiles - 1) / tiles;
+  const long long most = steps / 4;                                     // a split has 4 steps at least
+  if (want > most) want = most;
+  if (want > 64) want = 64;
+  if (want < 1) want = 1;
+  p.steps_per_split = dm_ceil_div(steps, want);
+  p.splits = dm_ceil_div(steps, p.steps_per_split);                     // no empty split
+  return p;
+}
+
+template <int T, int FORM>
+int launch16(const A8Args &a, unsigned grid, hipStream_t st) {
+  auto k = a8_gemm16_kernel<T, FORM, 2, 2, 2, 2>;
+  const size_t lds = 2 * (128 + 128) * 64 * 2;
+  k<<<grid, 256, lds, st>>>(a);
+  DM_CHECK_LAUNCH();
+  return DM_OK;
+}
+
+template <int FORM>
+int launch32(const A8Args &a, unsigned grid, hipStream_t st) {
+  a8_gemm32_kernel<FORM><<<grid, 256, (size_t)(3 * 128 * 32 + (FORM == 2 ? 1 : 3) * 128 * 32) * 2, st>>>(a);
+  DM_CHECK_LAUNCH();
+  return DM_OK;
+}
+
+template <int T>
+int reduce(const A8Args &a, hipStream_t st) {
+  const int col4 = dm_ceil_div(a.N, 32) * 8;
+  const long long main_blocks = ((long long)a.M * col4 + 255) / 256, more = a.rowsum ? (a.M + 255) / 256 : 0;
+  a8_reduce_kernel<T><<<(unsigned)(main_blocks + more), 256, 0, st>>>(a, col4, (unsigned)main_blocks);
+  DM_CHECK_LAUNCH();
+  return DM_OK;
+}
+
+}  // namespace
+
+extern "C" size_t dm_act8_gemm_workspace_bytes(int form, int dtype, int M, int N, int K) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  const Plan p = a8_plan(dtype, M, N, K);
+  return p.splits > 1 ? dm_align(((size_t)p.splits * M * N + (form == 2 ? (size_t)p.splits * M : 0)) * sizeof(float)) : 0;
+}
+
+extern "C" int dm_act8_gemm(int form, int dtype, const void *A, long long lda, const void *B, long long ldb, const uint8_t *exps,
+                            const void *bias, int relu, int M, int N, int K, void *C, uint32_t *sign_bits, void *rowsum,
+                            void *workspace, size_t workspace_bytes, dm_stream_t stream) {
+  hipStream_t st = (hipStream_t)stream;
+  if (form < 0 || form > 2 || dtype < ACT8_F32 || dtype > ACT8_F16 || M <= 0 || N <= 0 || K <= 0 || !A || !B || !C)
+    return DM_ERR_INVALID_ARG;
+  if ((form == 2) != (exps != nullptr) || (form != 2 && rowsum) || (form == 2 && (bias || relu || sign_bits))) return DM_ERR_INVALID_ARG;
+  if (lda < (form == 2 ? M : K) || ldb < (form == 0 ? K : N)) return DM_ERR_INVALID_ARG;
+  if (form == 2 && (ldb % 32 || ((uintptr_t)B & 15))) return DM_ERR_INVALID_ARG;
+  A8Args a = {};
+  if (dtype == ACT8_F32) {
+    a.vec_a = lda % 4 == 0 && ((uintptr_t)A & 15) == 0;
+    a.vec_b = ldb % 4 == 0 && ((uintptr_t)B & 15) == 0;
+  } else {
+    // 16-byte pieces: no piece crosses a row's end (the pitch has room for the last one), every address is a multiple of 16
+    if (lda % 8 || ((uintptr_t)A & 15) || (form != 2 && (ldb % 8 || ((uintptr_t)B & 15)))) return DM_ERR_UNSUPPORTED;
+  }
+  const Plan p = a8_plan(dtype, M, N, K);
+  a.A = A, a.B = B, a.bias = bias, a.exps = exps, a.C = C, a.bits = sign_bits, a.rowsum = rowsum;
+  a.M = M, a.N = N, a.K = K, a.lda = lda, a.ldb = ldb, a.relu = relu;
+  a.splits = p.splits, a.steps_per_split = p.steps_per_split, a.tiles_m = p.tiles_m, a.tiles_n = p.tiles_n;
+  a.vec_c = N % 4 == 0 && ((uintptr_t)C & 15) == 0;
+  if (p.splits > 1) {
+    if (!workspace || workspace_bytes < dm_act8_gemm_workspace_bytes(form, dtype, M, N, K)) return DM_ERR_WORKSPACE;
+    a.part = (float *)workspace;
+  }
+  const long long total = (long long)p.tiles_m * p.tiles_n * p.splits;
+  if (total > 0x3fffffff || (long long)M * (dm_ceil_div(N, 32) * 8) / 256 > 0x7ffffff0) return DM_ERR_INVALID_ARG;
+  a.per_xcd = (int)((total + 7) / 8);
+  const unsigned grid = (unsigned)a.per_xcd * 8;
+  int rc;
+  if (dtype == ACT8_F32) rc = form == 0 ? launch32<0>(a, grid, st) : form == 1 ? launch32<1>(a, grid, st) : launch32<2>(a, grid, st);
+  else if (dtype == ACT8_BF16)
+    rc = form == 0 ? launch16<ACT8_BF16, 0>(a, grid, st) : form == 1 ? launch16<ACT8_BF16, 1>(a, grid, st) : launch16<ACT8_BF16, 2>(a, grid, st);
+  else
+    rc = form == 0 ? launch16<ACT8_F16, 0>(a, grid, st) : form == 1 ? launch16<ACT8_F16, 1>(a, grid, st) : launch16<ACT8_F16, 2>(a, grid, st);
+  if (rc != DM_OK || p.splits == 1) return rc;
+  return dtype == ACT8_F32 ? reduce<ACT8_F32>(a, st) : dtype == ACT8_BF16 ? reduce<ACT8_BF16>(a, st) : reduce<ACT8_F16>(a, st);
+}
+
+extern "C" int dm_act8_mask_rows(const void *x, int dtype, long long rows, int width, long long ld, const uint32_t *sign_bits, void *out,
+                                 int ldo, dm_stream_t stream) {
+  if (dtype < ACT8_F32 || dtype > ACT8_F16 || rows < 0 || width <= 0 || ld < width || ldo < width || ldo % 8) return DM_ERR_INVALID_ARG;
+  if (rows == 0) return DM_OK;
+  if (!x || !out || ((uintptr_t)out & 15)) return DM_ERR_INVALID_ARG;
+  const int vec = ((uintptr_t)x & 15) == 0 && ld % (dtype == ACT8_F32 ? 4 : 8) == 0;
+  const long long blocks = (rows * (ldo / 8) + 255) / 256;
+  const unsigned grid = (unsigned)(blocks < 65536 ? blocks : 65536);
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == ACT8_F32) a8_mask_kernel<ACT8_F32><<<grid, 256, 0, st>>>(x, rows, width, ld, vec, sign_bits, out, ldo);
+  else if (dtype == ACT8_BF16) a8_mask_kernel<ACT8_BF16><<<grid, 256, 0, st>>>(x, rows, width, ld, vec, sign_bits, out, ldo);
+  else a8_mask_kernel<ACT8_F16><<<grid, 256, 0, st>>>(x, rows, width, ld, vec, sign_bits, out, ldo);
+  DM_CHECK_LAUNCH();
+  return DM_OK;
+}

@@ -1106,6 +1106,25 @@ int dm_act8_pack(const void *x, int dtype, long long rows, int width, long long 
 int dm_act8_unpack(const uint8_t *codes, const uint8_t *exps, long long rows, int width, void *out, int dtype,
                    dm_stream_t stream);
 
+/* The products of an FC layer whose weight gradient reads the 8-bit copy of its input.  One element type for A, B (forms 0, 1), bias, C
+ * and rowsum; accumulated in fp32 (fp32 operands: in three bf16 pieces each, 6 products; 3 with codes).
+ *   form 0  C[M][N] = A[M][K] . B[N][K]^T [+ bias[N]] [ReLU]   sign_bits (M, ceil(N / 32)) or NULL: bit n % 32 of word n / 32 = C > 0
+ *   form 1  C[M][N] = A[M][K] . B[K][N]
+ *   form 2  C[M][N] = A[K][M]^T . deq(B)[K][N]                 B codes, row pitch ldb = 32 * groups, exps (K, groups) as
+ *                                                              dm_act8_pack writes them; rowsum (M) or NULL: sums of A's columns
+ * Rows of A and B have pitches lda, ldb; C is dense.  16-bit operands: addresses multiples of 16 bytes, pitches of 8 elements
+ * (else DM_ERR_UNSUPPORTED), rows readable up to the next multiple of 8 elements, and 0 there where they run along the contraction
+ * (dm_act8_mask_rows without bits makes such a copy).  Few output tiles: the contraction is split and the parts (workspace) are
+ * added in order; results depend on shapes and values alone.
+ *   dm_act8_mask_rows  out (rows, ldo), ldo % 8 == 0: x where its sign bit is set (all of x without bits), 0 elsewhere and
+ *                      behind the width */
+size_t dm_act8_gemm_workspace_bytes(int form, int dtype, int M, int N, int K);
+int dm_act8_gemm(int form, int dtype, const void *A, long long lda, const void *B, long long ldb, const uint8_t *exps /*form 2*/,
+                 const void *bias /*or NULL*/, int relu, int M, int N, int K, void *C, uint32_t *sign_bits /*or NULL*/,
+                 void *rowsum /*or NULL*/, void *workspace, size_t workspace_bytes, dm_stream_t stream);
+int dm_act8_mask_rows(const void *x, int dtype, long long rows, int width, long long ld, const uint32_t *sign_bits /*or NULL*/,
+                      void *out, int ldo, dm_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

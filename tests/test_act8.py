@@ -56,3 +56,46 @@ def test_reference_rounding_agrees_with_torch():
     code, e = ref.pack(z)
     assert (e == 0).all()
     assert np.array_equal(code, z.float().to(torch.float8_e4m3fn).view(torch.uint8).numpy())
+
+
+def test_linear_refuses_what_it_cannot_take():
+    x, w = torch.zeros(4, 16), torch.zeros(8, 16)
+    with pytest.raises(_lib.DetMatchHipError):
+        act8.linear(x, w)
+    with pytest.raises(ValueError):
+        act8.linear(x, torch.zeros(8, 15))
+    with pytest.raises(ValueError):
+        act8.linear(x, w[0])
+    with pytest.raises(ValueError):
+        act8.linear(x, w, torch.zeros(7))
+    with pytest.raises(ValueError):
+        act8.linear(torch.zeros(4, 0), torch.zeros(8, 0))
+    with pytest.raises(TypeError):
+        act8.linear(x, w.half())
+    with pytest.raises(TypeError):
+        act8.linear(x.double(), w.double())
+    with pytest.raises(TypeError):
+        act8.linear(x, w, torch.zeros(8, dtype=torch.bfloat16))
+
+
+def test_gemm_entry_checks_its_arguments():
+    L = _lib.lib()
+    p = 4096                                  # an aligned address that no check looks behind
+    bad, unsupported, workspace = 1, 4, 2
+
+    def call(form=0, dtype=1, a=p, lda=64, b=p, ldb=64, exps=None, bias=None, relu=0, m=8, n=8, k=64, c=p, bits=None, rowsum=None):
+        return L.dm_act8_gemm(form, dtype, a, lda, b, ldb, exps, bias, relu, m, n, k, c, bits, rowsum, None, 0, None)
+
+    assert call(form=3) == bad and call(form=-1) == bad and call(dtype=3) == bad
+    assert call(m=0) == bad and call(n=-1) == bad and call(k=0) == bad
+    assert call(a=None) == bad and call(b=None) == bad and call(c=None) == bad
+    assert call(lda=63) == bad and call(ldb=56) == bad
+    assert call(form=2) == bad and call(exps=p) == bad and call(rowsum=p) == bad
+    assert call(form=2, exps=p, relu=1) == bad and call(form=2, exps=p, bias=p) == bad
+    assert call(form=2, exps=p, ldb=40) == bad and call(form=2, exps=p, b=p + 8) == bad
+    assert call(lda=68) == unsupported and call(a=p + 2) == unsupported and call(form=1, ldb=68) == unsupported
+    assert L.dm_act8_gemm_workspace_bytes(0, 1, 64, 64, 8192) > 0
+    assert call(lda=8192, ldb=8192, k=8192) == workspace
+    assert L.dm_act8_gemm_workspace_bytes(0, 1, 0, 64, 64) == 0
+    assert L.dm_act8_mask_rows(p, 1, 4, 12, 12, None, p, 12, None) == bad and L.dm_act8_mask_rows(p, 1, 4, 12, 8, None, p, 16, None) == bad
+    assert L.dm_act8_mask_rows(None, 1, 0, 12, 12, None, None, 16, None) == 0
