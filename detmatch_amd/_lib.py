@@ -29,6 +29,15 @@ class SpconvWgradJob(ctypes.Structure):
                 ('pair_stride', ci), ('kvol', ci), ('cin', ci), ('cout', ci)]
 
 
+class BlockNorm(ctypes.Structure):
+    """dm_block_norm (include/detmatch_hip.h)"""
+    _fields_ = [('dtype', ci), ('width', ci), ('rows', ctypes.c_longlong), ('layer', ci), ('post', ci), ('gate_act', ci),
+                ('param_f32', ci), ('scale_f32', ci), ('eps', cf), ('scale_host', cf), ('scale', vp), ('gate', vp),
+                ('ld_gate', ctypes.c_longlong), ('groups', ctypes.c_longlong), ('post_w', vp), ('post_b', vp), ('pre_w', vp),
+                ('pre_b', vp), ('f_mean', vp), ('f_rstd', vp), ('y_mean', vp), ('y_rstd', vp), ('f_codes', vp), ('f_exps', vp),
+                ('y_codes', vp), ('y_exps', vp)]
+
+
 # name -> (restype, argtypes); must list EVERY symbol include/detmatch_hip.h declares
 SIGNATURES = {
     'dm_version': (ctypes.c_char_p, []),
@@ -196,6 +205,11 @@ SIGNATURES = {
     'dm_act8_unpack': (ci, [vp, vp, ctypes.c_longlong, ci, vp, ci, vp]),
     'dm_act8_gemm_workspace_bytes': (sz, [ci, ci, ci, ci, ci]),
     'dm_act8_gemm': (ci, [ci, ci, vp, ctypes.c_longlong, vp, ctypes.c_longlong, vp, vp, ci, ci, ci, ci, vp, vp, vp, vp, sz, vp]),
+    'dm_block_norm_max_width': (ci, []),
+    'dm_block_norm_forward': (ci, [ctypes.POINTER(BlockNorm), vp, ctypes.c_longlong, vp, ctypes.c_longlong, vp, vp, vp]),
+    'dm_block_norm_workspace_bytes': (sz, [ctypes.c_longlong, ci, ctypes.c_longlong]),
+    'dm_block_norm_backward': (ci, [ctypes.POINTER(BlockNorm), vp, ctypes.c_longlong, vp, ctypes.c_longlong, vp, ctypes.c_longlong,
+                                    vp, ctypes.c_longlong, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]),
     'dm_act8_mask_rows': (ci, [vp, ci, ctypes.c_longlong, ci, ctypes.c_longlong, vp, vp, ci, vp]),
 }
 

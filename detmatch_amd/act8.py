@@ -139,11 +139,12 @@ def _gemm(form, code, a, b, exps, bias, relu, m, n, k, out, bits=None, rowsum=No
 class _Linear8(Function):
 
     @staticmethod
-    def forward(ctx, x, w, b, relu):
+    def forward(ctx, x, w, b, relu, grad):
+        # (grad: is autograd recording; inside of a Function it never is)
         code = DTYPES[x.dtype]
         m, k = x.shape
         n = w.shape[0]
-        needs = ctx.needs_input_grad
+        needs = ctx.needs_input_grad if grad else (False,) * 3
         with torch.cuda.device(x.device):
             y = torch.empty((m, n), dtype=x.dtype, device=x.device)
             bits = torch.empty((m, (n + 31) // 32), dtype=torch.int32, device=x.device) if relu and any(needs[:3]) else None
@@ -166,7 +167,7 @@ class _Linear8(Function):
         with torch.cuda.device(gy.device):
             if m == 0:
                 return (gy.new_zeros((0, k)) if need_x else None, gy.new_zeros((n, k)) if need_w else None,
-                        gy.new_zeros(n) if need_b else None, None)
+                        gy.new_zeros(n) if need_b else None, None, None)
             g = rows_view(gy)
             g = _operand(g, code) if bits is None else _masked(g, bits, code)
             if need_x:
@@ -181,7 +182,7 @@ class _Linear8(Function):
                     zero = torch.zeros((m, GROUP + 1), dtype=torch.uint8, device=gy.device)
                     _gemm(2, code, g, (zero[:, :GROUP].contiguous(), GROUP), zero[:, GROUP:].contiguous(), None, False, n, GROUP, m,
                           torch.empty((n, GROUP), dtype=gy.dtype, device=gy.device), rowsum=gb)
-        return gx, gw, gb, None
+        return gx, gw, gb, None, None
 
 
 def linear(x, w, b=None, relu=False):
@@ -204,4 +205,4 @@ def linear(x, w, b=None, relu=False):
     x2 = x.reshape(-1, x.shape[-1])
     if max(x2.shape[0], w.shape[0], w.shape[1]) > _MAX:
         raise ValueError('sizes up to %d are wanted, got x %s, w %s' % (_MAX, tuple(x.shape), tuple(w.shape)))
-    return _Linear8.apply(x2, w, b, bool(relu)).view(*x.shape[:-1], w.shape[0])
+    return _Linear8.apply(x2, w, b, bool(relu), torch.is_grad_enabled()).view(*x.shape[:-1], w.shape[0])

@@ -1125,6 +1125,42 @@ int dm_act8_gemm(int form, int dtype, const void *A, long long lda, const void *
 int dm_act8_mask_rows(const void *x, int dtype, long long rows, int width, long long ld, const uint32_t *sign_bits /*or NULL*/,
                       void *out, int ldo, dm_stream_t stream);
 
+/* ------------------------------------------------------------------------ */
+/* The norms around a residual block, fused with its gate and residual scale.  Rows of `width` channels (<= dm_block_norm_max_width()):
+ *   u = N(f) * post_w + post_b  (post == 0: u = f)     y = x + scale * act(gate) * u     h = N(y) * pre_w + pre_b
+ * N: RMS norm, or layer norm (`layer`); statistics and sums in fp32.  gate (groups, width): rows / groups consecutive rows share one row of
+ * gates.  f == NULL: h = N(x) * pre_w + pre_b alone (y == NULL, no gate).  h == NULL: no second norm.
+ * Forward writes, where the pointers are set, the statistics of f and y (means for the layer norm only) and 8-bit copies of f and of y as
+ * stored (dm_act8_pack's layout).  Backward takes the same struct, gradients gy, gh (one of them may be NULL), and f, y or their codes (a
+ * codes pointer wins); every output pointer may be NULL; dpre_* and dpost_* have the parameters' type, dscale the scale's, the others
+ * `dtype`.  rows == 0: DM_ERR_INVALID_ARG in the backward pass. */
+typedef struct dm_block_norm {
+  int dtype;            /* 0 fp32, 1 bf16, 2 fp16: x, f, gate, y, h and their gradients, dense outputs */
+  int width;
+  long long rows;
+  int layer;            /* 0 RMS norm, 1 layer norm */
+  int post;             /* is there a norm behind the block */
+  int gate_act;         /* 0 none, 1 sigmoid, 2 tanh */
+  int param_f32;        /* post_w, post_b, pre_w, pre_b are fp32 (else `dtype`) */
+  int scale_f32;        /* the number behind `scale` is fp32 (else `dtype`) */
+  float eps;
+  float scale_host;     /* the residual scale where `scale` is NULL */
+  const void *scale;
+  const void *gate;
+  long long ld_gate;
+  long long groups;     /* rows of gates; 0 without */
+  const void *post_w, *post_b, *pre_w, *pre_b;      /* (width) each; NULL: 1 resp. 0 */
+  float *f_mean, *f_rstd, *y_mean, *y_rstd;         /* (rows) */
+  uint8_t *f_codes, *f_exps, *y_codes, *y_exps;
+} dm_block_norm;
+int dm_block_norm_max_width(void);
+int dm_block_norm_forward(const dm_block_norm *q_host, const void *x, long long ldx, const void *f, long long ldf, void *y, void *h,
+                          dm_stream_t stream);
+size_t dm_block_norm_workspace_bytes(long long rows, int width, long long groups);
+int dm_block_norm_backward(const dm_block_norm *q_host, const void *gy, long long ldgy, const void *gh, long long ldgh, const void *y,
+                           long long ldy, const void *f, long long ldf, void *dx, void *df, void *dgate, void *dpre_w, void *dpre_b,
+                           void *dpost_w, void *dpost_b, void *dscale, void *workspace, size_t workspace_bytes, dm_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
