@@ -11,7 +11,7 @@ constexpr int A8_BLOCK = 256;
 // Bound by memory: element size in, 1 + 1/32 bytes out.
 template <int T>
 __global__ __launch_bounds__(A8_BLOCK) void act8_pack_kernel(const void *__restrict__ x, long long rows, int width, long long ld,
-                                                             int groups, int tpr, int vec, uint8_t *__restrict__ codes,
+                                                             int groups, int tpr, uint8_t *__restrict__ codes,
                                                              uint8_t *__restrict__ exps) {
   const int tx = threadIdx.x & (tpr - 1), ty = threadIdx.x / tpr, rpb = A8_BLOCK / tpr;
   const int chunks = groups * 4;
@@ -19,7 +19,7 @@ __global__ __launch_bounds__(A8_BLOCK) void act8_pack_kernel(const void *__restr
     for (int c = tx; c < chunks; c += tpr) {             // (chunks and tpr are multiples of 4: a quad stays together)
       float v[8];
       const int n = width - 8 * c;
-      act8_load8<T>(x, (size_t)r * ld + 8 * c, n, vec != 0, v);
+      act8_load8<T>(x, (size_t)r * ld + 8 * c, n, v);
       int e;
       const uint2 u = act8_encode8(v, &e);
       *(uint2 *)(codes + ((size_t)r * groups * ACT8_GROUP + 8 * c)) = u;
@@ -30,7 +30,7 @@ __global__ __launch_bounds__(A8_BLOCK) void act8_pack_kernel(const void *__restr
 
 template <int T>
 __global__ __launch_bounds__(A8_BLOCK) void act8_unpack_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ exps,
-                                                               long long rows, int width, int groups, int tpr, int vec,
+                                                               long long rows, int width, int groups, int tpr,
                                                                void *__restrict__ out) {
   const int tx = threadIdx.x & (tpr - 1), ty = threadIdx.x / tpr, rpb = A8_BLOCK / tpr;
   const int chunks = (width + 7) / 8;
@@ -44,7 +44,7 @@ __global__ __launch_bounds__(A8_BLOCK) void act8_unpack_kernel(const uint8_t *__
       act8_decode4(u.y, e, v + 4);
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] = v[k] != v[k] ? v[k] : fminf(fmaxf(v[k], -most), most);
-      act8_store8<T>(out, (size_t)r * width + 8 * c, width - 8 * c, vec != 0, v);
+      act8_store8<T>(out, (size_t)r * width + 8 * c, width - 8 * c, v);
     }
   }
 }
@@ -61,10 +61,6 @@ unsigned a8_grid(long long rows, int rpb) {
   return (unsigned)(b < 65536 ? b : 65536);
 }
 
-bool a8_aligned(const void *p, long long ld, int dtype) {
-  return ((uintptr_t)p & 15) == 0 && ld % (dtype == ACT8_F32 ? 4 : 8) == 0;
-}
-
 }  // namespace
 
 extern "C" int dm_act8_pack(const void *x, int dtype, long long rows, int width, long long ld, uint8_t *codes, uint8_t *exps,
@@ -73,12 +69,11 @@ extern "C" int dm_act8_pack(const void *x, int dtype, long long rows, int width,
   if (rows == 0) return DM_OK;
   if (!x || !codes || !exps || ((uintptr_t)codes & 7)) return DM_ERR_INVALID_ARG;
   const int groups = dm_ceil_div(width, ACT8_GROUP), tpr = a8_threads_per_row(groups * 4);
-  const int vec = a8_aligned(x, ld, dtype) ? 1 : 0;
   const unsigned grid = a8_grid(rows, A8_BLOCK / tpr);
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == ACT8_F32) act8_pack_kernel<ACT8_F32><<<grid, A8_BLOCK, 0, st>>>(x, rows, width, ld, groups, tpr, vec, codes, exps);
-  else if (dtype == ACT8_BF16) act8_pack_kernel<ACT8_BF16><<<grid, A8_BLOCK, 0, st>>>(x, rows, width, ld, groups, tpr, vec, codes, exps);
-  else act8_pack_kernel<ACT8_F16><<<grid, A8_BLOCK, 0, st>>>(x, rows, width, ld, groups, tpr, vec, codes, exps);
+  if (dtype == ACT8_F32) act8_pack_kernel<ACT8_F32><<<grid, A8_BLOCK, 0, st>>>(x, rows, width, ld, groups, tpr, codes, exps);
+  else if (dtype == ACT8_BF16) act8_pack_kernel<ACT8_BF16><<<grid, A8_BLOCK, 0, st>>>(x, rows, width, ld, groups, tpr, codes, exps);
+  else act8_pack_kernel<ACT8_F16><<<grid, A8_BLOCK, 0, st>>>(x, rows, width, ld, groups, tpr, codes, exps);
   DM_CHECK_LAUNCH();
   return DM_OK;
 }
@@ -89,12 +84,11 @@ extern "C" int dm_act8_unpack(const uint8_t *codes, const uint8_t *exps, long lo
   if (rows == 0) return DM_OK;
   if (!out || !codes || !exps || ((uintptr_t)codes & 7)) return DM_ERR_INVALID_ARG;
   const int groups = dm_ceil_div(width, ACT8_GROUP), tpr = a8_threads_per_row(dm_ceil_div(width, 8));
-  const int vec = a8_aligned(out, width, dtype) ? 1 : 0;
   const unsigned grid = a8_grid(rows, A8_BLOCK / tpr);
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == ACT8_F32) act8_unpack_kernel<ACT8_F32><<<grid, A8_BLOCK, 0, st>>>(codes, exps, rows, width, groups, tpr, vec, out);
-  else if (dtype == ACT8_BF16) act8_unpack_kernel<ACT8_BF16><<<grid, A8_BLOCK, 0, st>>>(codes, exps, rows, width, groups, tpr, vec, out);
-  else act8_unpack_kernel<ACT8_F16><<<grid, A8_BLOCK, 0, st>>>(codes, exps, rows, width, groups, tpr, vec, out);
+  if (dtype == ACT8_F32) act8_unpack_kernel<ACT8_F32><<<grid, A8_BLOCK, 0, st>>>(codes, exps, rows, width, groups, tpr, out);
+  else if (dtype == ACT8_BF16) act8_unpack_kernel<ACT8_BF16><<<grid, A8_BLOCK, 0, st>>>(codes, exps, rows, width, groups, tpr, out);
+  else act8_unpack_kernel<ACT8_F16><<<grid, A8_BLOCK, 0, st>>>(codes, exps, rows, width, groups, tpr, out);
   DM_CHECK_LAUNCH();
   return DM_OK;
 }

@@ -28,7 +28,7 @@ __device__ __forceinline__ int act8_exponent(float amax) {
   return e < -127 ? -127 : e;                                                       // (subnormal amax: e = -135 or -134 -> -127)
 }
 
-// four codes of x * inv (inv = 2^-e), lowest byte first
+// four codes of x * inv (inv = 2^-e), lowest byte first, whatever the values are
 __device__ __forceinline__ uint32_t act8_encode4(float a, float b, float c, float d, float inv, float limit) {
   int r = __builtin_amdgcn_cvt_pk_fp8_f32(fminf(fmaxf(a * inv, -limit), limit), fminf(fmaxf(b * inv, -limit), limit), 0, false);
   r = __builtin_amdgcn_cvt_pk_fp8_f32(fminf(fmaxf(c * inv, -limit), limit), fminf(fmaxf(d * inv, -limit), limit), r, true);
@@ -38,6 +38,11 @@ __device__ __forceinline__ uint32_t act8_encode4(float a, float b, float c, floa
   if (!act8_finite(c)) u = (u & 0xff00ffffu) | 0x7f0000u;
   if (!act8_finite(d)) u = (u & 0x00ffffffu) | 0x7f000000u;
   return u;
+}
+
+// the same where the products are at most 448 or nan: the instruction's own rounding, nan -> nan
+__device__ __forceinline__ uint32_t act8_encode4_fast(float a, float b, float c, float d, float inv) {
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c * inv, d * inv, __builtin_amdgcn_cvt_pk_fp8_f32(a * inv, b * inv, 0, false), true);
 }
 
 __device__ __forceinline__ float act8_limit(int e) { return e >= 120 ? 240.f : 448.f; }
@@ -51,13 +56,16 @@ __device__ __forceinline__ void act8_decode4(uint32_t u, int e, float *v) {
 }
 
 // ---- 8 consecutive elements of a row, any element type --------------------------------------------------------------
+// Rows of any pitch: the global loads and stores of gfx950 take 16 bytes at any address of the element's alignment, at full rate
+// where it is a multiple of 16.
+typedef uint32_t act8_u32x4 __attribute__((ext_vector_type(4)));
+typedef act8_u32x4 act8_u32x4_any __attribute__((aligned(2)));
+typedef __bf16 act8_bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 act8_f16x2 __attribute__((ext_vector_type(2)));
+
 __device__ __forceinline__ float act8_bf16_f32(uint32_t h) { return __uint_as_float(h << 16); }
 
-__device__ __forceinline__ uint16_t act8_f32_bf16(float v) {       // round to nearest even, nan kept
-  const uint32_t b = __float_as_uint(v);
-  if ((b & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((b >> 16) | 0x40u);
-  return (uint16_t)((b + 0x7fffu + ((b >> 16) & 1u)) >> 16);
-}
+__device__ __forceinline__ uint16_t act8_f32_bf16(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }   // to nearest even
 
 template <int T>
 __device__ __forceinline__ float act8_get(const void *p, size_t i) {
@@ -73,58 +81,106 @@ __device__ __forceinline__ void act8_put(void *p, size_t i, float v) {
   else ((_Float16 *)p)[i] = (_Float16)v;
 }
 
-// n (1 .. 8) elements from p + i on; the rest 0.  vec: i and the row are 16-byte aligned (then n < 8 only at a row's end)
+// 8 elements as they lie in memory
 template <int T>
-__device__ __forceinline__ void act8_load8(const void *p, size_t i, int n, bool vec, float *v) {
-  if (vec && n >= 8) {
-    if constexpr (T == ACT8_F32) {
-      const float4 a = *(const float4 *)((const float *)p + i), b = *(const float4 *)((const float *)p + i + 4);
-      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+struct Act8Raw {
+  act8_u32x4 w[T == ACT8_F32 ? 2 : 1];
+};
+
+// n elements from p + i on (none where n <= 0, 8 where n >= 8); the rest 0
+template <int T>
+__device__ __forceinline__ Act8Raw<T> act8_load_raw(const void *p, size_t i, int n) {
+  Act8Raw<T> r;
+  if constexpr (T == ACT8_F32) {
+    const float *q = (const float *)p + i;
+    if (n >= 8) {
+      r.w[0] = *(const act8_u32x4_any *)q, r.w[1] = *(const act8_u32x4_any *)(q + 4);
     } else {
-      const uint4 a = *(const uint4 *)((const uint16_t *)p + i);
-      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if constexpr (T == ACT8_BF16) {
-          v[2 * k] = __uint_as_float(w[k] << 16), v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
-        } else {
-          union { uint32_t u; _Float16 h[2]; } c;
-          c.u = w[k];
-          v[2 * k] = (float)c.h[0], v[2 * k + 1] = (float)c.h[1];
-        }
-      }
+      for (int k = 0; k < 8; ++k) r.w[k / 4][k % 4] = k < n ? __float_as_uint(q[k]) : 0u;
     }
-    return;
-  }
+  } else {
+    const uint16_t *q = (const uint16_t *)p + i;
+    if (n >= 8) {
+      r.w[0] = *(const act8_u32x4_any *)q;
+    } else {
 #pragma unroll
-  for (int k = 0; k < 8; ++k) v[k] = k < n ? act8_get<T>(p, i + k) : 0.f;
+      for (int k = 0; k < 4; ++k) r.w[0][k] = (2 * k < n ? (uint32_t)q[2 * k] : 0u) | (2 * k + 1 < n ? (uint32_t)q[2 * k + 1] << 16 : 0u);
+    }
+  }
+  return r;
 }
 
 template <int T>
-__device__ __forceinline__ void act8_store8(void *p, size_t i, int n, bool vec, const float *v) {
-  if (vec && n >= 8) {
-    if constexpr (T == ACT8_F32) {
-      *(float4 *)((float *)p + i) = make_float4(v[0], v[1], v[2], v[3]);
-      *(float4 *)((float *)p + i + 4) = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-      uint32_t w[4];
+__device__ __forceinline__ void act8_unraw(const Act8Raw<T> &r, float *v) {
+  if constexpr (T == ACT8_F32) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if constexpr (T == ACT8_BF16) {
-          w[k] = (uint32_t)act8_f32_bf16(v[2 * k]) | ((uint32_t)act8_f32_bf16(v[2 * k + 1]) << 16);
-        } else {
-          union { uint32_t u; _Float16 h[2]; } c;
-          c.h[0] = (_Float16)v[2 * k], c.h[1] = (_Float16)v[2 * k + 1];
-          w[k] = c.u;
-        }
+    for (int k = 0; k < 8; ++k) v[k] = __uint_as_float(r.w[k / 4][k % 4]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t w = r.w[0][k];
+      if constexpr (T == ACT8_BF16) v[2 * k] = __uint_as_float(w << 16), v[2 * k + 1] = __uint_as_float(w & 0xffff0000u);
+      else {
+        const act8_f16x2 h = __builtin_bit_cast(act8_f16x2, w);
+        v[2 * k] = (float)h[0], v[2 * k + 1] = (float)h[1];
       }
-      *(uint4 *)((uint16_t *)p + i) = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    return;
   }
+}
+
+template <int T>
+__device__ __forceinline__ Act8Raw<T> act8_raw(const float *v) {
+  Act8Raw<T> r;
+  if constexpr (T == ACT8_F32) {
 #pragma unroll
-  for (int k = 0; k < 8; ++k)
-    if (k < n) act8_put<T>(p, i + k, v[k]);
+    for (int k = 0; k < 8; ++k) r.w[k / 4][k % 4] = __float_as_uint(v[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (T == ACT8_BF16) {
+        act8_bf16x2 h = {(__bf16)v[2 * k], (__bf16)v[2 * k + 1]};
+        r.w[0][k] = __builtin_bit_cast(uint32_t, h);
+      } else {
+        act8_f16x2 h = {(_Float16)v[2 * k], (_Float16)v[2 * k + 1]};
+        r.w[0][k] = __builtin_bit_cast(uint32_t, h);
+      }
+    }
+  }
+  return r;
+}
+
+template <int T>
+__device__ __forceinline__ void act8_store_raw(void *p, size_t i, int n, const Act8Raw<T> &r) {
+  if constexpr (T == ACT8_F32) {
+    float *q = (float *)p + i;
+    if (n >= 8) {
+      *(act8_u32x4_any *)q = r.w[0], *(act8_u32x4_any *)(q + 4) = r.w[1];
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k < n) q[k] = __uint_as_float(r.w[k / 4][k % 4]);
+    }
+  } else {
+    uint16_t *q = (uint16_t *)p + i;
+    if (n >= 8) {
+      *(act8_u32x4_any *)q = r.w[0];
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k < n) q[k] = (uint16_t)(r.w[0][k / 2] >> (16 * (k & 1)));
+    }
+  }
+}
+
+template <int T>
+__device__ __forceinline__ void act8_load8(const void *p, size_t i, int n, float *v) {
+  act8_unraw<T>(act8_load_raw<T>(p, i, n), v);
+}
+
+template <int T>
+__device__ __forceinline__ void act8_store8(void *p, size_t i, int n, const float *v) {
+  act8_store_raw<T>(p, i, n, act8_raw<T>(v));
 }
 
 // largest finite value of an element type: what unpacking saturates at (2^16 is a code's value, but not fp16's)
@@ -135,18 +191,36 @@ __device__ __forceinline__ float act8_most() {
   else return 65504.f;
 }
 
-// a group is 4 neighbouring threads with 8 elements each: maximum over them, by lane exchange inside the quad
+// lane exchange inside 4 neighbouring lanes
+template <int CTRL>
+__device__ __forceinline__ float act8_dpp(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+
+enum { ACT8_DPP_XOR1 = 0xB1, ACT8_DPP_XOR2 = 0x4E, ACT8_DPP_HALF_MIRROR = 0x141, ACT8_DPP_MIRROR = 0x140 };
+
+// a group is 4 neighbouring threads with 8 elements each: maximum over them
 __device__ __forceinline__ float act8_quad_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 1));
-  return fmaxf(v, __shfl_xor(v, 2));
+  v = fmaxf(v, act8_dpp<ACT8_DPP_XOR1>(v));
+  return fmaxf(v, act8_dpp<ACT8_DPP_XOR2>(v));
 }
 
 // 8 values of one thread of a quad -> 8 codes; *e_out = the group's exponent.  All 4 threads of the quad take part.
 __device__ __forceinline__ uint2 act8_encode8(const float *v, int *e_out) {
   float m = 0.f;
 #pragma unroll
+  for (int k = 0; k < 8; k += 2) asm("v_max3_f32 %0, |%1|, |%2|, %0" : "+v"(m) : "v"(v[k]), "v"(v[k + 1]));
+  m = act8_quad_max(m);
+  int e = act8_exponent(m);
+  if (act8_finite(m) && e < 120) {               // (a nan beside finite values does not show in m; it becomes a nan all the same)
+    const float inv = act8_2exp(-e);
+    *e_out = e;
+    return make_uint2(act8_encode4_fast(v[0], v[1], v[2], v[3], inv), act8_encode4_fast(v[4], v[5], v[6], v[7], inv));
+  }
+  m = 0.f;
+#pragma unroll
   for (int k = 0; k < 8; ++k) m = fmaxf(m, act8_finite_abs(v[k]));
-  const int e = act8_exponent(act8_quad_max(m));
+  e = act8_exponent(act8_quad_max(m));
   const float inv = act8_2exp(-e), limit = act8_limit(e);
   *e_out = e;
   return make_uint2(act8_encode4(v[0], v[1], v[2], v[3], inv, limit), act8_encode4(v[4], v[5], v[6], v[7], inv, limit));

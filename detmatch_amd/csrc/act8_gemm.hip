@@ -34,7 +34,7 @@ struct A8Args {
   void *rowsum;               // form 2: sum over the contraction of A's columns (M)
   int M, N, K;
   long long lda, ldb;
-  int relu, splits, steps_per_split, tiles_m, tiles_n, per_xcd, vec_a, vec_b, vec_c;
+  int relu, splits, steps_per_split, tiles_m, tiles_n, per_xcd, vec_c;
 };
 
 // ---- where a 16-byte piece of a staged tile lies in LDS ----------------------------------------------------------------
@@ -176,7 +176,7 @@ struct F32Regs {
 
 template <bool ALONG_K, int ROWS, int BK, int THREADS>
 __device__ __forceinline__ void fetch_f32(F32Regs<ROWS, BK, THREADS> &t, const float *P, long long ld, int row0, int rows, int k0, int k_hi,
-                                          int tid, bool vec) {
+                                          int tid) {
 #pragma unroll
   for (int h = 0; h < F32Regs<ROWS, BK, THREADS>::H; ++h) {
     const int i = tid + THREADS * h;
@@ -191,7 +191,7 @@ __device__ __forceinline__ void fetch_f32(F32Regs<ROWS, BK, THREADS> &t, const f
       n = k < k_hi ? rows - row : 0;
       at = (long long)k * ld + row;
     }
-    act8_load8<ACT8_F32>(P, (size_t)at, n, vec, t.v[h]);
+    act8_load8<ACT8_F32>(P, (size_t)at, n, t.v[h]);
   }
 }
 
@@ -418,9 +418,9 @@ __global__ __launch_bounds__(256) void a8_gemm32_kernel(A8Args a) {
   CodeRegs<BN, BK, THREADS> codes;
 
   auto fetch = [&](int s) {
-    fetch_f32<FORM == 2, BM, BK, THREADS>(ra, (const float *)a.A, a.lda, m0, a.M, s * BK, a.K, tid, a.vec_a != 0);
+    fetch_f32<FORM == 2, BM, BK, THREADS>(ra, (const float *)a.A, a.lda, m0, a.M, s * BK, a.K, tid);
     if constexpr (FORM == 2) fetch_codes<BN, BK, THREADS>(codes, (const uint8_t *)a.B, a.exps, a.ldb, n0, s * BK, a.K, tid);
-    else fetch_f32<FORM == 1, BN, BK, THREADS>(rb, (const float *)a.B, a.ldb, n0, a.N, s * BK, a.K, tid, a.vec_b != 0);
+    else fetch_f32<FORM == 1, BN, BK, THREADS>(rb, (const float *)a.B, a.ldb, n0, a.N, s * BK, a.K, tid);
   };
 
   if (s_lo < s_hi) fetch(s_lo);
@@ -531,7 +531,7 @@ __global__ __launch_bounds__(256) void a8_reduce_kernel(A8Args a, int col4, unsi
 // ---- a gradient behind a ReLU / rows moved to a 16-byte pitch --------------------------------------------------------------
 // out (rows, ldo) = bits ? (bit set ? x : 0) : x, 0 behind the width; a thread has 8 elements
 template <int T>
-__global__ __launch_bounds__(256) void a8_mask_kernel(const void *__restrict__ x, long long rows, int width, long long ld, int vec,
+__global__ __launch_bounds__(256) void a8_mask_kernel(const void *__restrict__ x, long long rows, int width, long long ld,
                                                       const uint32_t *__restrict__ bits, void *__restrict__ out, int ldo) {
   const int chunks = ldo / 8;
   const long long total = rows * chunks;
@@ -539,13 +539,13 @@ __global__ __launch_bounds__(256) void a8_mask_kernel(const void *__restrict__ x
     const long long r = i / chunks;
     const int c = 8 * (int)(i % chunks);
     float v[8];
-    act8_load8<T>(x, (size_t)r * ld + c, width - c, vec != 0, v);
+    act8_load8<T>(x, (size_t)r * ld + c, width - c, v);
     if (bits && c < width) {
       const uint32_t w = bits[r * ((width + 31) / 32) + c / 32] >> (c & 31);
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] = (w >> k) & 1 ? v[k] : 0.f;
     }
-    act8_store8<T>(out, (size_t)r * ldo + c, 8, true, v);
+    act8_store8<T>(out, (size_t)r * ldo + c, 8, v);
   }
 }
 
@@ -613,10 +613,7 @@ extern "C" int dm_act8_gemm(int form, int dtype, const void *A, long long lda, c
   if (lda < (form == 2 ? M : K) || ldb < (form == 0 ? K : N)) return DM_ERR_INVALID_ARG;
   if (form == 2 && (ldb % 32 || ((uintptr_t)B & 15))) return DM_ERR_INVALID_ARG;
   A8Args a = {};
-  if (dtype == ACT8_F32) {
-    a.vec_a = lda % 4 == 0 && ((uintptr_t)A & 15) == 0;
-    a.vec_b = ldb % 4 == 0 && ((uintptr_t)B & 15) == 0;
-  } else {
+  if (dtype != ACT8_F32) {
     // 16-byte pieces: no piece crosses a row's end (the pitch has room for the last one), every address is a multiple of 16
     if (lda % 8 || ((uintptr_t)A & 15) || (form != 2 && (ldb % 8 || ((uintptr_t)B & 15)))) return DM_ERR_UNSUPPORTED;
   }
@@ -648,13 +645,12 @@ extern "C" int dm_act8_mask_rows(const void *x, int dtype, long long rows, int w
   if (dtype < ACT8_F32 || dtype > ACT8_F16 || rows < 0 || width <= 0 || ld < width || ldo < width || ldo % 8) return DM_ERR_INVALID_ARG;
   if (rows == 0) return DM_OK;
   if (!x || !out || ((uintptr_t)out & 15)) return DM_ERR_INVALID_ARG;
-  const int vec = ((uintptr_t)x & 15) == 0 && ld % (dtype == ACT8_F32 ? 4 : 8) == 0;
   const long long blocks = (rows * (ldo / 8) + 255) / 256;
   const unsigned grid = (unsigned)(blocks < 65536 ? blocks : 65536);
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == ACT8_F32) a8_mask_kernel<ACT8_F32><<<grid, 256, 0, st>>>(x, rows, width, ld, vec, sign_bits, out, ldo);
-  else if (dtype == ACT8_BF16) a8_mask_kernel<ACT8_BF16><<<grid, 256, 0, st>>>(x, rows, width, ld, vec, sign_bits, out, ldo);
-  else a8_mask_kernel<ACT8_F16><<<grid, 256, 0, st>>>(x, rows, width, ld, vec, sign_bits, out, ldo);
+  if (dtype == ACT8_F32) a8_mask_kernel<ACT8_F32><<<grid, 256, 0, st>>>(x, rows, width, ld, sign_bits, out, ldo);
+  else if (dtype == ACT8_BF16) a8_mask_kernel<ACT8_BF16><<<grid, 256, 0, st>>>(x, rows, width, ld, sign_bits, out, ldo);
+  else a8_mask_kernel<ACT8_F16><<<grid, 256, 0, st>>>(x, rows, width, ld, sign_bits, out, ldo);
   DM_CHECK_LAUNCH();
   return DM_OK;
 }

@@ -27,9 +27,10 @@ struct BnArgs {
   uint8_t *f_codes, *f_exps, *y_codes, *y_exps;  // ... or codes of f and y
   float *f_mean, *f_rstd, *y_mean, *y_rstd;      // statistics (rows); means only for the layer norm
   float *part;                                   // backward: sums per workgroup [set][blocks][C], then [blocks] of the scale's
-  long long rows, each, groups, ldx, ldf, ldg, ldgy, ldgh;
-  float eps, scale_host;
-  int C, T, act, post, w32, s32, vx, vf, vg, vgy, vgh, vw, vo, by_unit, n_blocks;
+  long long ldx, ldf, ldg, ldgy, ldgh;
+  uint32_t rows, each, groups;                   // groups of `each` rows
+  float eps, scale_host, inv_c;
+  int C, T, act, post, w32, s32, by_unit, n_blocks, sets;   // sets: which sums over rows are wanted, a bit each
 };
 
 enum { ACT_NONE = 0, ACT_SIGMOID = 1, ACT_TANH = 2 };
@@ -37,7 +38,7 @@ enum { ACT_NONE = 0, ACT_SIGMOID = 1, ACT_TANH = 2 };
 enum { SET_PRE_W = 0, SET_PRE_B = 1, SET_POST_W = 2, SET_POST_B = 3, SET_GATE = 4, SETS = 5 };
 
 __device__ __forceinline__ float act_of(int act, float z) {
-  if (act == ACT_SIGMOID) return 1.f / (1.f + expf(-z));
+  if (act == ACT_SIGMOID) return __builtin_amdgcn_rcpf(1.f + __expf(-z));
   if (act == ACT_TANH) return tanhf(z);
   return z;
 }
@@ -46,13 +47,28 @@ __device__ __forceinline__ float act_slope(int act, float g) {      // from the 
   return act == ACT_SIGMOID ? g * (1.f - g) : act == ACT_TANH ? 1.f - g * g : 1.f;
 }
 
-// sums of NV numbers over a team; `red` holds two sets of partial sums in turn, so one barrier a call is enough: a set is
-// written again only after the barrier of the call in between
+__device__ __forceinline__ float rsqrt_of(float v) {                 // (the instruction takes no subnormal numbers)
+  return v < 1e-30f ? __builtin_amdgcn_rsqf(v * 0x1p64f) * 0x1p32f : __builtin_amdgcn_rsqf(v);
+}
+
+// sums of NV numbers over a team: lane exchanges inside a wave (every lane ends with the same sum), LDS between waves.  `red` holds two sets of
+// partial sums in turn, so one barrier a call is enough: a set is written again only after the barrier of the call in between.
 template <int NV>
 __device__ __forceinline__ void team_sum(float (&v)[NV], int T, float *red, int &turn) {
-  for (int o = (T < 64 ? T : 64) >> 1; o; o >>= 1) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) v[i] += __shfl_xor(v[i], o);
+  for (int i = 0; i < NV; ++i) {
+    v[i] += act8_dpp<ACT8_DPP_XOR1>(v[i]);
+    v[i] += act8_dpp<ACT8_DPP_XOR2>(v[i]);
+    v[i] += act8_dpp<ACT8_DPP_HALF_MIRROR>(v[i]);
+    if (T >= 16) v[i] += act8_dpp<ACT8_DPP_MIRROR>(v[i]);
+    if (T >= 32) {
+      const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]), __float_as_uint(v[i]), false, false);
+      v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    if (T >= 64) {
+      const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(v[i]), false, false);
+      v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
   }
   if (T > 64) {
     float *r = red + turn * 32;
@@ -78,8 +94,8 @@ __device__ __forceinline__ void load_param(const BnArgs &a, const void *p, int c
   if (!p) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = absent;
-  } else if (a.w32) act8_load8<ACT8_F32>(p, c, a.C - c, a.vw != 0, v);
-  else act8_load8<T>(p, c, a.C - c, a.vw != 0, v);
+  } else if (a.w32) act8_load8<ACT8_F32>(p, c, a.C - c, v);
+  else act8_load8<T>(p, c, a.C - c, v);
 }
 
 template <int T>
@@ -88,29 +104,42 @@ __device__ __forceinline__ float load_scale(const BnArgs &a) {
   return a.s32 ? *(const float *)a.scale : act8_get<T>(a.scale, 0);
 }
 
+// 8 codes of a row and their exponent, in the place of the 8 elements they stand for
 template <int T>
-__device__ __forceinline__ float rounded(float v) {
-  if constexpr (T == ACT8_F32) return v;
-  else if constexpr (T == ACT8_BF16) return act8_bf16_f32(act8_f32_bf16(v));
-  else return (float)(_Float16)v;
+__device__ __forceinline__ Act8Raw<T> load_codes(const uint8_t *codes, const uint8_t *exps, size_t row, int groups, int c, int n) {
+  Act8Raw<T> r;
+  r.w[0] = act8_u32x4{0u, 0u, 127u, 0u};
+  if (n > 0) {
+    const uint2 u = *(const uint2 *)(codes + (row * groups * ACT8_GROUP + c));
+    r.w[0].x = u.x, r.w[0].y = u.y, r.w[0].z = exps[row * groups + c / ACT8_GROUP];
+  }
+  return r;
 }
 
-// the values that 8 codes of a row stand for in the element type
 template <int T>
-__device__ __forceinline__ void load_codes(const uint8_t *codes, const uint8_t *exps, size_t row, int groups, int c, float *v) {
-  const uint2 u = *(const uint2 *)(codes + (row * groups * ACT8_GROUP + c));
-  const int e = (int)exps[row * groups + c / ACT8_GROUP] - 127;
-  act8_decode4(u.x, e, v), act8_decode4(u.y, e, v + 4);
-  if constexpr (T == ACT8_F16) {
+__device__ __forceinline__ void unraw_codes(const Act8Raw<T> &r, float *v) {
+  const int e = (int)r.w[0].z - 127;
+  act8_decode4(r.w[0].x, e, v), act8_decode4(r.w[0].y, e, v + 4);
+  if constexpr (T == ACT8_F16) {                     // (the other types hold every code exactly)
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = v[k] != v[k] ? v[k] : rounded<T>(fminf(fmaxf(v[k], -65504.f), 65504.f));
+    for (int k = 0; k < 8; ++k) v[k] = v[k] != v[k] ? v[k] : (float)(_Float16)fminf(fmaxf(v[k], -65504.f), 65504.f);
   }
 }
 
-// mean and 1 / deviation of the row held by a team (values behind the width are 0); fixed two-step form: the deviation is taken around the
-// mean, not from a difference of squares
+__device__ __forceinline__ void store_codes8(const float *v, uint8_t *codes, uint8_t *exps, size_t row, int groups, int c, bool live) {
+  int e;
+  const uint2 w = act8_encode8(v, &e);
+  if (live && c < groups * ACT8_GROUP) {
+    *(uint2 *)(codes + (row * groups * ACT8_GROUP + c)) = w;
+    if ((threadIdx.x & 3) == 0) exps[row * groups + c / ACT8_GROUP] = (uint8_t)(e + 127);
+  }
+}
+
+// mean and 1 / deviation of the row held by a team (values behind the width are 0); the deviation is taken around the mean, not from a
+// difference of squares
 template <bool LAYER, int NCH>
-__device__ __forceinline__ void row_stats(const BnArgs &a, float (&v)[NCH][8], int tx, float *red, int &turn, float *mean, float *rstd) {
+__device__ __forceinline__ void row_stats(const BnArgs &a, const float (&v)[NCH][8], int tx, float *red, int &turn, float *mean,
+                                          float *rstd) {
   float s[1] = {0.f};
   *mean = 0.f;
   if constexpr (LAYER) {
@@ -119,7 +148,7 @@ __device__ __forceinline__ void row_stats(const BnArgs &a, float (&v)[NCH][8], i
 #pragma unroll
       for (int k = 0; k < 8; ++k) s[0] += v[n][k];
     team_sum<1>(s, a.T, red, turn);
-    *mean = s[0] / (float)a.C;
+    *mean = s[0] * a.inv_c;
     s[0] = 0.f;
   }
 #pragma unroll
@@ -127,44 +156,66 @@ __device__ __forceinline__ void row_stats(const BnArgs &a, float (&v)[NCH][8], i
     const int left = a.C - 8 * (tx + n * a.T);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const float d = k < left ? v[n][k] - *mean : 0.f;
+      const float d = LAYER ? (k < left ? v[n][k] - *mean : 0.f) : v[n][k];
       s[0] = fmaf(d, d, s[0]);
     }
   }
   team_sum<1>(s, a.T, red, turn);
-  *rstd = 1.f / sqrtf(s[0] / (float)a.C + a.eps);
+  *rstd = rsqrt_of(fmaf(s[0], a.inv_c, a.eps));
 }
 
+// A workgroup's teams walk the rows with the grid's stride.  The next row's operands are under way while this one is computed.
 template <int T, bool LAYER, int NCH, int BLOCK>
 __global__ __launch_bounds__(BLOCK) void block_norm_fwd_kernel(BnArgs a) {
   __shared__ float red[64];
   const int tx = threadIdx.x & (a.T - 1), team = threadIdx.x / a.T, teams = BLOCK / a.T, groups8 = (a.C + 31) / 32;
   int turn = 0;
   const float scale = load_scale<T>(a);
-  for (long long r0 = (long long)blockIdx.x * teams; r0 < a.rows; r0 += (long long)gridDim.x * teams) {
-    const long long row = r0 + team;
-    const bool live = row < a.rows;                 // (all teams of a workgroup take part in the sums)
-    float y[NCH][8], u[NCH][8];
+  const bool has_f = a.f != nullptr, gate_each = a.gate && a.groups > 1;
+  float post_w[NCH][8], post_b[LAYER ? NCH : 1][8], pre_w[NCH][8], pre_b[LAYER ? NCH : 1][8], g[NCH][8];
+#pragma unroll
+  for (int n = 0; n < NCH; ++n) {
+    const int c = 8 * (tx + n * a.T);
+    load_param<T>(a, a.post_w, c, post_w[n], 1.f), load_param<T>(a, a.pre_w, c, pre_w[n], 1.f);
+    if constexpr (LAYER) load_param<T>(a, a.post_b, c, post_b[n], 0.f), load_param<T>(a, a.pre_b, c, pre_b[n], 0.f);
+    if (a.gate && !gate_each) {
+      act8_load8<T>(a.gate, c, a.C - c, g[n]);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) g[n][k] = act_of(a.act, g[n][k]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) g[n][k] = 1.f;
+    }
+  }
+  struct In {
+    Act8Raw<T> x[NCH], f[NCH], g[NCH];
+  } next;
+  auto fetch = [&](uint32_t row) {
 #pragma unroll
     for (int n = 0; n < NCH; ++n) {
-      const int c = 8 * (tx + n * a.T), left = live ? a.C - c : 0;
-      act8_load8<T>(a.x, (size_t)row * a.ldx + c, left, a.vx != 0, y[n]);
-      if (a.f) act8_load8<T>(a.f, (size_t)row * a.ldf + c, left, a.vf != 0, u[n]);
+      const int c = 8 * (tx + n * a.T), left = row < a.rows ? a.C - c : 0;
+      next.x[n] = act8_load_raw<T>(a.x, (size_t)row * a.ldx + c, left);
+      if (has_f) next.f[n] = act8_load_raw<T>(a.f, (size_t)row * a.ldf + c, left);
+      if (gate_each) next.g[n] = act8_load_raw<T>(a.gate, (size_t)(a.each == 1 ? row : row / a.each) * a.ldg + c, left);
     }
-    if (a.f) {
-      if (a.f_codes) {
+  };
+  const uint32_t stride = gridDim.x * teams;
+  fetch(blockIdx.x * teams + team);
+  for (uint32_t r0 = blockIdx.x * teams; r0 < a.rows; r0 += stride) {
+    const uint32_t row = r0 + team;
+    const bool live = row < a.rows;                 // (all teams of a workgroup take part in the sums)
+    const In in = next;
+    fetch(row + stride);
+    float y[NCH][8];
 #pragma unroll
-        for (int n = 0; n < NCH; ++n) {
-          const int c = 8 * (tx + n * a.T);
-          int e;
-          const uint2 w = act8_encode8(u[n], &e);
-          if (live && c < groups8 * 32) {
-            *(uint2 *)(a.f_codes + ((size_t)row * groups8 * 32 + c)) = w;
-            if ((tx & 3) == 0) a.f_exps[(size_t)row * groups8 + c / 32] = (uint8_t)(e + 127);
-          }
-        }
+    for (int n = 0; n < NCH; ++n) act8_unraw<T>(in.x[n], y[n]);
+    if (has_f) {
+      float u[NCH][8], mean = 0.f, rstd = 1.f;
+#pragma unroll
+      for (int n = 0; n < NCH; ++n) {
+        act8_unraw<T>(in.f[n], u[n]);
+        if (a.f_codes) store_codes8(u[n], a.f_codes, a.f_exps, row, groups8, 8 * (tx + n * a.T), live);
       }
-      float mean = 0.f, rstd = 1.f;
       if (a.post) {
         row_stats<LAYER, NCH>(a, u, tx, red, turn, &mean, &rstd);
         if (live && tx == 0 && a.f_rstd) {
@@ -176,37 +227,34 @@ __global__ __launch_bounds__(BLOCK) void block_norm_fwd_kernel(BnArgs a) {
       for (int n = 0; n < NCH; ++n) {
         const int c = 8 * (tx + n * a.T);
         if (a.post) {
-          float w[8], b[8];
-          load_param<T>(a, a.post_w, c, w, 1.f);
-          load_param<T>(a, a.post_b, c, b, 0.f);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) u[n][k] = fmaf((u[n][k] - mean) * rstd, w[k], b[k]);
+          for (int k = 0; k < 8; ++k) {
+            if constexpr (LAYER) u[n][k] = fmaf((u[n][k] - mean) * rstd, post_w[n][k], post_b[n][k]);
+            else u[n][k] = u[n][k] * rstd * post_w[n][k];
+          }
         }
-        if (a.gate) {
-          float g[8];
-          act8_load8<T>(a.gate, (size_t)(row / a.each) * a.ldg + c, live ? a.C - c : 0, a.vg != 0, g);
+        if (gate_each) {
+          act8_unraw<T>(in.g[n], g[n]);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) u[n][k] *= act_of(a.act, g[k]);
+          for (int k = 0; k < 8; ++k) g[n][k] = act_of(a.act, g[n][k]);
         }
 #pragma unroll
-        for (int k = 0; k < 8; ++k) y[n][k] = c + k < a.C ? fmaf(scale, u[n][k], y[n][k]) : 0.f;
-        if (live && a.y) act8_store8<T>(a.y, (size_t)row * a.C + c, a.C - c, a.vo != 0, y[n]);
-      }
-    }
-    if (a.y_codes) {
+        for (int k = 0; k < 8; ++k) y[n][k] = fmaf(scale, g[n][k] * u[n][k], y[n][k]);
+        if (c + 8 > a.C) {                          // (gates and biases behind the width leave no trace)
 #pragma unroll
-      for (int n = 0; n < NCH; ++n) {
-        const int c = 8 * (tx + n * a.T);
-        float v[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = rounded<T>(y[n][k]);
-        int e;
-        const uint2 w = act8_encode8(v, &e);
-        if (live && c < groups8 * 32) {
-          *(uint2 *)(a.y_codes + ((size_t)row * groups8 * 32 + c)) = w;
-          if ((tx & 3) == 0) a.y_exps[(size_t)row * groups8 + c / 32] = (uint8_t)(e + 127);
+          for (int k = 0; k < 8; ++k) y[n][k] = c + k < a.C ? y[n][k] : 0.f;
+        }
+        const Act8Raw<T> stored = act8_raw<T>(y[n]);
+        if (live && a.y) act8_store_raw<T>(a.y, (size_t)row * a.C + c, a.C - c, stored);
+        if (a.y_codes) {                            // of y as it is stored
+          float v[8];
+          act8_unraw<T>(stored, v);
+          store_codes8(v, a.y_codes, a.y_exps, row, groups8, c, live);
         }
       }
+    } else if (a.y_codes) {
+#pragma unroll
+      for (int n = 0; n < NCH; ++n) store_codes8(y[n], a.y_codes, a.y_exps, row, groups8, 8 * (tx + n * a.T), live);
     }
     if (a.h) {
       float mean, rstd;
@@ -218,12 +266,12 @@ __global__ __launch_bounds__(BLOCK) void block_norm_fwd_kernel(BnArgs a) {
 #pragma unroll
       for (int n = 0; n < NCH; ++n) {
         const int c = 8 * (tx + n * a.T);
-        float w[8], b[8];
-        load_param<T>(a, a.pre_w, c, w, 1.f);
-        load_param<T>(a, a.pre_b, c, b, 0.f);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) w[k] = fmaf((y[n][k] - mean) * rstd, w[k], b[k]);
-        if (live) act8_store8<T>(a.h, (size_t)row * a.C + c, a.C - c, a.vo != 0, w);
+        for (int k = 0; k < 8; ++k) {
+          if constexpr (LAYER) y[n][k] = fmaf((y[n][k] - mean) * rstd, pre_w[n][k], pre_b[n][k]);
+          else y[n][k] = y[n][k] * rstd * pre_w[n][k];
+        }
+        if (live) act8_store8<T>(a.h, (size_t)row * a.C + c, a.C - c, y[n]);
       }
     }
   }
@@ -234,170 +282,199 @@ __global__ __launch_bounds__(BLOCK) void block_norm_fwd_kernel(BnArgs a) {
 template <int T, bool LAYER, int NCH, int BLOCK>
 __global__ __launch_bounds__(BLOCK) void block_norm_bwd_kernel(BnArgs a) {
   __shared__ float red[64];
-  __shared__ float sums[BLOCK <= 256 ? 256 * 8 : 1];
+  __shared__ float sums[BLOCK <= 512 ? BLOCK * 8 : 1];
   const int tx = threadIdx.x & (a.T - 1), team = threadIdx.x / a.T, teams = BLOCK / a.T, groups8 = (a.C + 31) / 32;
   int turn = 0;
   const float scale = load_scale<T>(a);
+  const bool has_f = a.f || a.f_codes, has_h = a.gh != nullptr;
   float acc[SETS][NCH][8], dscale = 0.f;
+  float post_w[NCH][8], post_b[LAYER ? NCH : 1][8], pre_w[NCH][8], g[NCH][8];
 #pragma unroll
-  for (int s = 0; s < SETS; ++s)
+  for (int n = 0; n < NCH; ++n) {
+    const int c = 8 * (tx + n * a.T);
+    load_param<T>(a, a.post_w, c, post_w[n], 1.f), load_param<T>(a, a.pre_w, c, pre_w[n], 1.f);
+    if constexpr (LAYER) load_param<T>(a, a.post_b, c, post_b[n], 0.f);
 #pragma unroll
-    for (int n = 0; n < NCH; ++n)
+    for (int k = 0; k < 8; ++k) {
+      g[n][k] = 1.f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) acc[s][n][k] = 0.f;
-  const long long stride = (long long)gridDim.x * teams, first = (long long)blockIdx.x * teams + team;
-  const long long trips = a.by_unit ? (a.groups + stride - 1) / stride * a.each : (a.each + stride - 1) / stride;
-  long long unit = first, in_unit = 0;
-  for (long long i = 0; i < trips; ++i) {
-    long long row;
-    bool live;
-    if (a.by_unit) {
-      live = unit < a.groups;
-      row = unit * a.each + in_unit;
-    } else {
-      const long long r = first + i * stride;
-      live = r < a.each;
-      row = (long long)blockIdx.y * a.each + r;
+      for (int s = 0; s < SETS; ++s) acc[s][n][k] = 0.f;
     }
-    const long long gate_row = a.by_unit ? unit : blockIdx.y;
+  }
+  const uint32_t stride = gridDim.x * teams, first = blockIdx.x * teams + team;
+  const uint32_t trips = a.by_unit ? (a.groups + stride - 1) / stride * a.each : (a.each + stride - 1) / stride;
+  struct In {
+    Act8Raw<T> gh[NCH], gy[NCH], y[NCH], f[NCH], g[NCH];
+    float y_mean, y_rstd, f_mean, f_rstd;
+    uint32_t row, unit;
+    bool live, last;              // last: the group's last row
+  } next;
+  uint32_t unit = a.by_unit ? first : blockIdx.y, in_unit = a.by_unit ? 0 : first;
+  auto fetch = [&]() {
+    next.live = unit < a.groups && in_unit < a.each;
+    next.row = unit * a.each + in_unit, next.unit = unit;
+    next.last = a.by_unit && in_unit + 1 == a.each;
+    const size_t row = next.row;
+    next.y_mean = next.y_rstd = next.f_mean = next.f_rstd = 0.f;
+    if (next.live) {
+      if (has_h) {
+        next.y_rstd = a.y_rstd[row];
+        if (LAYER) next.y_mean = a.y_mean[row];
+      }
+      if (has_f && a.post) {
+        next.f_rstd = a.f_rstd[row];
+        if (LAYER) next.f_mean = a.f_mean[row];
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NCH; ++n) {
+      const int c = 8 * (tx + n * a.T), left = next.live ? a.C - c : 0;
+      if (has_h) {
+        next.gh[n] = act8_load_raw<T>(a.gh, row * a.ldgh + c, left);
+        if (a.y_codes) next.y[n] = load_codes<T>(a.y_codes, a.y_exps, row, groups8, c, left);
+        else next.y[n] = act8_load_raw<T>(a.y_in, row * a.ldx + c, left);
+      }
+      if (a.gy) next.gy[n] = act8_load_raw<T>(a.gy, row * a.ldgy + c, left);
+      if (has_f) {
+        if (a.f_codes) next.f[n] = load_codes<T>(a.f_codes, a.f_exps, row, groups8, c, left);
+        else next.f[n] = act8_load_raw<T>(a.f, row * a.ldf + c, left);
+        if (a.gate) next.g[n] = act8_load_raw<T>(a.gate, (size_t)unit * a.ldg + c, left);
+      }
+    }
+    if (!a.by_unit) in_unit += stride;
+    else if (++in_unit == a.each) in_unit = 0, unit += stride;
+  };
+  if (trips) fetch();
+  for (uint32_t i = 0; i < trips; ++i) {
+    const In in = next;
+    if (i + 1 < trips) fetch();
     float dy[NCH][8];
 #pragma unroll
     for (int n = 0; n < NCH; ++n) {
-      const int c = 8 * (tx + n * a.T);
-      if (a.gy) act8_load8<T>(a.gy, (size_t)row * a.ldgy + c, live ? a.C - c : 0, a.vgy != 0, dy[n]);
+      if (a.gy) act8_unraw<T>(in.gy[n], dy[n]);
       else
 #pragma unroll
         for (int k = 0; k < 8; ++k) dy[n][k] = 0.f;
     }
-    if (a.gh) {
+    // (channels behind the width, and rows of a team without one: gradients are 0 there, and what multiplies them is finite)
+    if (has_h) {
       float hat[NCH][8], d[NCH][8], s[2] = {0.f, 0.f};
-      const float rstd = live ? a.y_rstd[row] : 0.f, mean = LAYER && live ? a.y_mean[row] : 0.f;
 #pragma unroll
       for (int n = 0; n < NCH; ++n) {
-        const int c = 8 * (tx + n * a.T), left = live ? a.C - c : 0;
-        float w[8];
-        act8_load8<T>(a.gh, (size_t)row * a.ldgh + c, left, a.vgh != 0, d[n]);
-        if (a.y_codes) {
-          if (left > 0) load_codes<T>(a.y_codes, a.y_exps, (size_t)row, groups8, c, hat[n]);
-          else
-#pragma unroll
-            for (int k = 0; k < 8; ++k) hat[n][k] = 0.f;
-        } else act8_load8<T>(a.y_in, (size_t)row * a.ldx + c, left, a.vx != 0, hat[n]);
-        load_param<T>(a, a.pre_w, c, w, 1.f);
+        act8_unraw<T>(in.gh[n], d[n]);
+        if (a.y_codes) unraw_codes<T>(in.y[n], hat[n]);
+        else act8_unraw<T>(in.y[n], hat[n]);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          hat[n][k] = k < left ? (hat[n][k] - mean) * rstd : 0.f;
+          if (LAYER) hat[n][k] -= in.y_mean;
+          hat[n][k] *= in.y_rstd;
           acc[SET_PRE_W][n][k] = fmaf(d[n][k], hat[n][k], acc[SET_PRE_W][n][k]);
           if (LAYER) acc[SET_PRE_B][n][k] += d[n][k];
-          d[n][k] = k < left ? d[n][k] * w[k] : 0.f;
+          d[n][k] *= pre_w[n][k];
           s[0] = fmaf(d[n][k], hat[n][k], s[0]);
-          s[1] += d[n][k];
+          if (LAYER) s[1] += d[n][k];
         }
       }
       if constexpr (LAYER) team_sum<2>(s, a.T, red, turn);
       else {
         float one[1] = {s[0]};
         team_sum<1>(one, a.T, red, turn);
-        s[0] = one[0], s[1] = 0.f;
+        s[0] = one[0];
       }
-      const float m0 = s[0] / (float)a.C, m1 = s[1] / (float)a.C;
+      const float m0 = s[0] * a.inv_c, m1 = s[1] * a.inv_c;
 #pragma unroll
       for (int n = 0; n < NCH; ++n)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) dy[n][k] = fmaf(rstd, d[n][k] - m1 - hat[n][k] * m0, dy[n][k]);
+        for (int k = 0; k < 8; ++k) {
+          if (LAYER) d[n][k] -= m1;
+          dy[n][k] = fmaf(in.y_rstd, fmaf(-hat[n][k], m0, d[n][k]), dy[n][k]);
+        }
     }
 #pragma unroll
     for (int n = 0; n < NCH; ++n) {
       const int c = 8 * (tx + n * a.T);
-      if (live && a.dx) act8_store8<T>(a.dx, (size_t)row * a.C + c, a.C - c, a.vo != 0, dy[n]);
+      if (in.live && a.dx) act8_store8<T>(a.dx, (size_t)in.row * a.C + c, a.C - c, dy[n]);
     }
-    if (a.f || a.f_codes) {
+    if (has_f) {
       float hat[NCH][8], s[2] = {0.f, 0.f};
-      float rstd = 1.f, mean = 0.f;
-      if (a.post) {
-        rstd = live ? a.f_rstd[row] : 0.f;
-        if (LAYER && live) mean = a.f_mean[row];
-      }
 #pragma unroll
       for (int n = 0; n < NCH; ++n) {
-        const int c = 8 * (tx + n * a.T), left = live ? a.C - c : 0;
-        float w[8], b[8], g[8];
-        if (a.f_codes) {
-          if (left > 0) load_codes<T>(a.f_codes, a.f_exps, (size_t)row, groups8, c, hat[n]);
-          else
+        const int c = 8 * (tx + n * a.T);
+        if (c + 8 > a.C) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) hat[n][k] = 0.f;
-        } else act8_load8<T>(a.f, (size_t)row * a.ldf + c, left, a.vf != 0, hat[n]);
-        if (a.post) {
-          load_param<T>(a, a.post_w, c, w, 1.f);
-          load_param<T>(a, a.post_b, c, b, 0.f);
+          for (int k = 0; k < 8; ++k) dy[n][k] = c + k < a.C ? dy[n][k] : 0.f;
         }
-        if (a.gate) act8_load8<T>(a.gate, (size_t)gate_row * a.ldg + c, left, a.vg != 0, g);
+        if (a.f_codes) unraw_codes<T>(in.f[n], hat[n]);
+        else act8_unraw<T>(in.f[n], hat[n]);
+        if (a.gate) {
+          act8_unraw<T>(in.g[n], g[n]);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) g[n][k] = act_of(a.act, g[n][k]);
+        }
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          float u = hat[n][k];
+          float u = hat[n][k], t = dy[n][k];
           if (a.post) {
-            hat[n][k] = k < left ? (hat[n][k] - mean) * rstd : 0.f;
-            u = fmaf(hat[n][k], w[k], b[k]);
+            if (LAYER) hat[n][k] -= in.f_mean;
+            hat[n][k] *= in.f_rstd;
+            u = LAYER ? fmaf(hat[n][k], post_w[n][k], post_b[n][k]) : hat[n][k] * post_w[n][k];
           }
-          const float up = k < left ? dy[n][k] : 0.f, gk = a.gate ? act_of(a.act, g[k]) : 1.f;
-          dscale = fmaf(up * gk, k < left ? u : 0.f, dscale);
-          float t = up * scale;
-          if (a.gate) acc[SET_GATE][n][k] = fmaf(t, k < left ? u : 0.f, acc[SET_GATE][n][k]);
-          t *= gk;
+          const float tu = t * u;
+          dscale = fmaf(tu, g[n][k], dscale);
+          if (a.gate) acc[SET_GATE][n][k] += tu;
+          t *= g[n][k];
           if (a.post) {
             acc[SET_POST_W][n][k] = fmaf(t, hat[n][k], acc[SET_POST_W][n][k]);
-            if (LAYER) acc[SET_POST_B][n][k] += k < left ? t : 0.f;
-            t = k < left ? t * w[k] : 0.f;
+            if (LAYER) acc[SET_POST_B][n][k] += t;
+            t *= post_w[n][k];
             s[0] = fmaf(t, hat[n][k], s[0]);
-            s[1] += t;
+            if (LAYER) s[1] += t;
           }
           dy[n][k] = t;
         }
       }
+      float r = scale;
       if (a.post) {
         if constexpr (LAYER) team_sum<2>(s, a.T, red, turn);
         else {
           float one[1] = {s[0]};
           team_sum<1>(one, a.T, red, turn);
-          s[0] = one[0], s[1] = 0.f;
+          s[0] = one[0];
         }
-        const float m0 = s[0] / (float)a.C, m1 = s[1] / (float)a.C;
+        const float m0 = s[0] * a.inv_c, m1 = s[1] * a.inv_c;
+        r *= in.f_rstd;
 #pragma unroll
         for (int n = 0; n < NCH; ++n)
 #pragma unroll
-          for (int k = 0; k < 8; ++k) dy[n][k] = rstd * (dy[n][k] - m1 - hat[n][k] * m0);
+          for (int k = 0; k < 8; ++k) {
+            if (LAYER) dy[n][k] -= m1;
+            dy[n][k] = fmaf(-hat[n][k], m0, dy[n][k]);
+          }
       }
 #pragma unroll
       for (int n = 0; n < NCH; ++n) {
         const int c = 8 * (tx + n * a.T);
-        if (live && a.df) act8_store8<T>(a.df, (size_t)row * a.C + c, a.C - c, a.vo != 0, dy[n]);
-      }
-    }
-    if (a.by_unit && ++in_unit == a.each) {            // this group of rows is done: its gates' gradient is complete
-      if (a.gate) {
 #pragma unroll
-        for (int n = 0; n < NCH; ++n) {
-          const int c = 8 * (tx + n * a.T), left = live ? a.C - c : 0;
-          float g[8];
-          act8_load8<T>(a.gate, (size_t)unit * a.ldg + c, left, a.vg != 0, g);
+        for (int k = 0; k < 8; ++k) dy[n][k] *= r;
+        if (in.live && a.df) act8_store8<T>(a.df, (size_t)in.row * a.C + c, a.C - c, dy[n]);
+        if (in.last && a.gate) {                     // this group of rows is done: its gates' gradient is complete
+          float v[8];
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            g[k] = acc[SET_GATE][n][k] * act_slope(a.act, act_of(a.act, g[k]));
+            v[k] = acc[SET_GATE][n][k] * scale * act_slope(a.act, g[n][k]);
             acc[SET_GATE][n][k] = 0.f;
           }
-          if (live && a.dgate) act8_store8<T>(a.dgate, (size_t)unit * a.C + c, left, a.vo != 0, g);
+          if (in.live && a.dgate) act8_store8<T>(a.dgate, (size_t)in.unit * a.C + c, a.C - c, v);
         }
       }
-      in_unit = 0, unit += stride;
     }
   }
-  // this workgroup's sums
+  // this workgroup's sums; the residual scale, the same for all, is multiplied on when they are added up
   const size_t block = (size_t)blockIdx.y * gridDim.x + blockIdx.x;
-  if (BLOCK <= 256 && teams > 1) {
+  if (BLOCK <= 512 && teams > 1) {
 #pragma unroll
     for (int s = 0; s < SETS; ++s) {
-      if (s == SET_GATE && a.by_unit) continue;
+      if (!((a.sets >> s) & 1)) continue;
       __syncthreads();
 #pragma unroll
       for (int k = 0; k < 8; ++k) sums[threadIdx.x * 8 + k] = acc[s][0][k];
@@ -411,12 +488,11 @@ __global__ __launch_bounds__(BLOCK) void block_norm_bwd_kernel(BnArgs a) {
   } else {
 #pragma unroll
     for (int s = 0; s < SETS; ++s) {
-      if (s == SET_GATE && a.by_unit) continue;
+      if (!((a.sets >> s) & 1)) continue;
 #pragma unroll
       for (int n = 0; n < NCH; ++n) {
         const int c = 8 * (tx + n * a.T);
-        for (int k = 0; k < 8; ++k)
-          if (c + k < a.C) a.part[((size_t)s * a.n_blocks + block) * a.C + c + k] = acc[s][n][k];
+        act8_store8<ACT8_F32>(a.part, ((size_t)s * a.n_blocks + block) * a.C + c, a.C - c, acc[s][n]);
       }
     }
   }
@@ -429,42 +505,53 @@ __global__ __launch_bounds__(BLOCK) void block_norm_bwd_kernel(BnArgs a) {
 struct SumArgs {
   const float *part;
   void *out[SETS], *dscale;
-  const void *gate;
+  const void *gate, *scale;
   long long ldg;
+  float scale_host;
   int C, act, n_blocks, groups, w32, s32;
 };
 
-// sums over the workgroups, in order: 64 columns x 4 slices of the workgroups; blockIdx.y: set (gates: set + group)
+// Sums over the workgroups, in a fixed order: 32 columns x 32 slices of the workgroups, 8 loads of a thread under way at a time;
+// blockIdx.y: set (gates: set + group).  Bound by the latency of the loads of a slice: few workgroups have little to read.
 template <int T>
-__global__ __launch_bounds__(256) void block_norm_sum_kernel(SumArgs a) {
-  __shared__ float sh[4][64];
-  const int lane = threadIdx.x & 63, slice = threadIdx.x >> 6;
-  if (blockIdx.x * 64 >= (unsigned)a.C) {              // the workgroup behind the columns: the scale's gradient
-    if (blockIdx.y || !a.dscale) return;
-    float v = 0.f;
-    for (int b = threadIdx.x; b < a.n_blocks; b += 256) v += a.part[(size_t)SETS * a.n_blocks * a.C + b];
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    if (lane == 0) sh[0][slice] = v;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      v = (sh[0][0] + sh[0][1]) + (sh[0][2] + sh[0][3]);
-      if (a.s32) *(float *)a.dscale = v;
-      else act8_put<T>(a.dscale, 0, v);
-    }
-    return;
-  }
+__global__ __launch_bounds__(1024) void block_norm_sum_kernel(SumArgs a) {
+  __shared__ float sh[32][33];
+  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
+  const bool last = blockIdx.x * 32 >= (unsigned)a.C;    // the workgroup behind the columns: the scale's gradient
   const int set = min((int)blockIdx.y, (int)SET_GATE), group = (int)blockIdx.y - set;
-  if (!a.out[set]) return;
-  const int c = blockIdx.x * 64 + lane;
-  const int blocks = set == SET_GATE ? a.n_blocks / a.groups : a.n_blocks;
-  const float *p = a.part + ((size_t)set * a.n_blocks + (size_t)group * blocks) * a.C + c;
+  if (last ? blockIdx.y || !a.dscale : !a.out[set]) return;
+  const int c = blockIdx.x * 32 + lane, blocks = set == SET_GATE ? a.n_blocks / a.groups : a.n_blocks;
+  const float *p;
+  size_t step;
+  int b, n;
+  if (last) p = a.part + (size_t)SETS * a.n_blocks * a.C, step = 1, b = threadIdx.x, n = 1024;
+  else p = a.part + ((size_t)set * a.n_blocks + (size_t)group * blocks) * a.C + c, step = a.C, b = slice, n = 32;
   float v = 0.f;
-  if (c < a.C)
-    for (int b = slice; b < blocks; b += 4) v += p[(size_t)b * a.C];
+  if (last || c < a.C) {
+    for (; b + 7 * n < blocks; b += 8 * n) {
+      float w[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) w[k] = p[(size_t)(b + k * n) * step];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v += w[k];
+    }
+    for (; b < blocks; b += n) v += p[(size_t)b * step];
+  }
   sh[slice][lane] = v;
   __syncthreads();
-  if (slice || c >= a.C) return;
-  v = (sh[0][lane] + sh[1][lane]) + (sh[2][lane] + sh[3][lane]);
+  if (slice) return;
+  v = 0.f;
+#pragma unroll
+  for (int k = 0; k < 32; ++k) v += sh[k][lane];
+  if (last) {
+    for (int o = 16; o; o >>= 1) v += __shfl_xor(v, o);
+    if (lane) return;
+    if (a.s32) *(float *)a.dscale = v;
+    else act8_put<T>(a.dscale, 0, v);
+    return;
+  }
+  if (c >= a.C) return;
+  if (set >= SET_POST_W) v *= !a.scale ? a.scale_host : a.s32 ? *(const float *)a.scale : act8_get<T>(a.scale, 0);
   if (set == SET_GATE) {
     v *= act_slope(a.act, act_of(a.act, act8_get<T>(a.gate, (size_t)group * a.ldg + c)));
     act8_put<T>(a.out[set], (size_t)group * a.C + c, v);
@@ -483,7 +570,7 @@ bool bn_plan(int C, BnPlan *p) {
   if (chunks > 2 * t) t <<= 1;
   p->T = t;
   p->nch = dm_ceil_div(chunks, t);
-  p->block = t <= 256 ? 256 : t;
+  p->block = t <= 512 ? 512 : t;
   return p->nch <= 2;
 }
 
@@ -493,8 +580,7 @@ struct BnGrid {
 };
 
 BnGrid bn_grid(const BnPlan &p, long long rows, long long groups) {
-  const int teams = p.block / p.T;
-  const int most = p.block >= 1024 ? 512 : p.block >= 512 ? 768 : 1024;
+  const int teams = p.block / p.T, most = 512;      // two workgroups a compute unit: each of them leaves sums behind
   BnGrid g;
   g.by_unit = groups > 64;
   const long long units = g.by_unit ? groups : rows / (groups > 0 ? groups : 1);
@@ -507,10 +593,9 @@ BnGrid bn_grid(const BnPlan &p, long long rows, long long groups) {
 template <int T, bool LAYER>
 int launch_fwd(const BnArgs &a, const BnPlan &p, hipStream_t st) {
   const int teams = p.block / p.T;
-  const long long blocks = (a.rows + teams - 1) / teams;
-  const unsigned grid = (unsigned)(blocks < 16384 ? blocks : 16384);
-  if (p.block == 256) block_norm_fwd_kernel<T, LAYER, 1, 256><<<grid, 256, 0, st>>>(a);
-  else if (p.block == 512 && p.nch == 1) block_norm_fwd_kernel<T, LAYER, 1, 512><<<grid, 512, 0, st>>>(a);
+  const uint32_t blocks = (a.rows + teams - 1) / teams, most = 1024;   // (as many as are resident at once, and parameters are read once)
+  const unsigned grid = blocks < most ? blocks : most;
+  if (p.block == 512 && p.nch == 1) block_norm_fwd_kernel<T, LAYER, 1, 512><<<grid, 512, 0, st>>>(a);
   else if (p.block == 512) block_norm_fwd_kernel<T, LAYER, 2, 512><<<grid, 512, 0, st>>>(a);
   else block_norm_fwd_kernel<T, LAYER, 2, 1024><<<grid, 1024, 0, st>>>(a);
   DM_CHECK_LAUNCH();
@@ -520,21 +605,16 @@ int launch_fwd(const BnArgs &a, const BnPlan &p, hipStream_t st) {
 template <int T, bool LAYER>
 int launch_bwd(const BnArgs &a, const BnPlan &p, const BnGrid &g, hipStream_t st) {
   const dim3 grid(g.x, g.y);
-  if (p.block == 256) block_norm_bwd_kernel<T, LAYER, 1, 256><<<grid, 256, 0, st>>>(a);
-  else if (p.block == 512 && p.nch == 1) block_norm_bwd_kernel<T, LAYER, 1, 512><<<grid, 512, 0, st>>>(a);
+  if (p.block == 512 && p.nch == 1) block_norm_bwd_kernel<T, LAYER, 1, 512><<<grid, 512, 0, st>>>(a);
   else if (p.block == 512) block_norm_bwd_kernel<T, LAYER, 2, 512><<<grid, 512, 0, st>>>(a);
   else block_norm_bwd_kernel<T, LAYER, 2, 1024><<<grid, 1024, 0, st>>>(a);
   DM_CHECK_LAUNCH();
   return DM_OK;
 }
 
-int vec_of(const void *p, long long ld, int dtype) {
-  return ((uintptr_t)p & 15) == 0 && ld % (dtype == ACT8_F32 ? 4 : 8) == 0;
-}
-
 // what forward and backward have in common; returns a DM_ERR_* code
 int fill(BnArgs *a, const dm_block_norm *q, BnPlan *p) {
-  if (!q || q->dtype < ACT8_F32 || q->dtype > ACT8_F16 || q->rows < 0 || q->width <= 0) return DM_ERR_INVALID_ARG;
+  if (!q || q->dtype < ACT8_F32 || q->dtype > ACT8_F16 || q->rows < 0 || q->rows > 0x7ffffc00 || q->width <= 0) return DM_ERR_INVALID_ARG;
   if (!bn_plan(q->width, p)) return DM_ERR_UNSUPPORTED;
   if (q->gate_act < ACT_NONE || q->gate_act > ACT_TANH || q->groups < 0 || (q->gate ? q->groups < 1 || q->rows % q->groups : q->groups != 0))
     return DM_ERR_INVALID_ARG;
@@ -542,11 +622,9 @@ int fill(BnArgs *a, const dm_block_norm *q, BnPlan *p) {
   if (!(q->eps >= 0.f)) return DM_ERR_INVALID_ARG;
   const int dt = q->dtype;
   a->gate = q->gate, a->post_w = q->post_w, a->post_b = q->post_b, a->pre_w = q->pre_w, a->pre_b = q->pre_b, a->scale = q->scale;
-  a->rows = q->rows, a->groups = q->groups, a->each = q->groups > 0 ? q->rows / q->groups : q->rows;
-  a->ldg = q->ld_gate, a->eps = q->eps, a->scale_host = q->scale_host, a->C = q->width, a->T = p->T;
+  a->rows = (uint32_t)q->rows, a->groups = q->groups > 0 ? (uint32_t)q->groups : 1, a->each = a->rows / a->groups;
+  a->ldg = q->ld_gate, a->inv_c = 1.f / (float)q->width, a->eps = q->eps, a->scale_host = q->scale_host, a->C = q->width, a->T = p->T;
   a->act = q->gate_act, a->post = q->post, a->w32 = q->param_f32 || dt == ACT8_F32, a->s32 = q->scale_f32 || dt == ACT8_F32;
-  a->vg = vec_of(q->gate, q->ld_gate, dt);
-  a->vw = !(((uintptr_t)q->post_w | (uintptr_t)q->post_b | (uintptr_t)q->pre_w | (uintptr_t)q->pre_b) & 15);
   a->f_mean = q->f_mean, a->f_rstd = q->f_rstd, a->y_mean = q->y_mean, a->y_rstd = q->y_rstd;
   a->f_codes = q->f_codes, a->f_exps = q->f_exps, a->y_codes = q->y_codes, a->y_exps = q->y_exps;
   if ((!q->f_codes != !q->f_exps) || (!q->y_codes != !q->y_exps) || (((uintptr_t)q->f_codes | (uintptr_t)q->y_codes) & 7)) return DM_ERR_INVALID_ARG;
@@ -568,8 +646,6 @@ extern "C" int dm_block_norm_forward(const dm_block_norm *q, const void *x, long
   const bool layer = q->layer != 0;
   if (layer && ((a.f_rstd && !a.f_mean) || (a.y_rstd && !a.y_mean))) return DM_ERR_INVALID_ARG;
   a.x = x, a.f = f, a.y = y, a.h = h, a.ldx = ldx, a.ldf = ldf;
-  a.vx = vec_of(x, ldx, q->dtype), a.vf = vec_of(f, ldf, q->dtype);
-  a.vo = !(((uintptr_t)y | (uintptr_t)h) & 15) && q->width % (q->dtype == ACT8_F32 ? 4 : 8) == 0;
   hipStream_t st = (hipStream_t)stream;
   if (q->dtype == ACT8_F32) return layer ? launch_fwd<ACT8_F32, true>(a, p, st) : launch_fwd<ACT8_F32, false>(a, p, st);
   if (q->dtype == ACT8_BF16) return layer ? launch_fwd<ACT8_BF16, true>(a, p, st) : launch_fwd<ACT8_BF16, false>(a, p, st);
@@ -602,11 +678,10 @@ extern "C" int dm_block_norm_backward(const dm_block_norm *q, const void *gy, lo
   const int dt = q->dtype;
   a.gy = gy, a.gh = gh, a.y_in = y, a.f = f, a.ldgy = ldgy, a.ldgh = ldgh, a.ldx = ldy, a.ldf = ldf;
   a.dx = dx, a.df = df, a.dgate = dgate, a.part = (float *)workspace;
-  a.vgy = vec_of(gy, ldgy, dt), a.vgh = vec_of(gh, ldgh, dt), a.vx = vec_of(y, ldy, dt), a.vf = vec_of(f, ldf, dt);
-  a.vo = !(((uintptr_t)dx | (uintptr_t)df | (uintptr_t)dgate) & 15) && q->width % (dt == ACT8_F32 ? 4 : 8) == 0;
   const BnGrid g = bn_grid(p, q->rows, q->groups);
   a.by_unit = g.by_unit, a.n_blocks = g.x * g.y;
-  if (q->groups == 0) a.groups = 1;
+  a.sets = (dpre_w ? 1 << SET_PRE_W : 0) | (dpre_b ? 1 << SET_PRE_B : 0) | (dpost_w ? 1 << SET_POST_W : 0) | (dpost_b ? 1 << SET_POST_B : 0) |
+           (dgate && !g.by_unit ? 1 << SET_GATE : 0);
   hipStream_t st = (hipStream_t)stream;
   int e;
   if (dt == ACT8_F32) e = layer ? launch_bwd<ACT8_F32, true>(a, p, g, st) : launch_bwd<ACT8_F32, false>(a, p, g, st);
@@ -615,14 +690,14 @@ extern "C" int dm_block_norm_backward(const dm_block_norm *q, const void *gy, lo
   if (e != DM_OK) return e;
   SumArgs s = {};
   s.part = a.part, s.dscale = dscale, s.gate = q->gate, s.ldg = q->ld_gate, s.C = q->width, s.act = q->gate_act, s.n_blocks = a.n_blocks;
-  s.groups = g.y, s.w32 = a.w32, s.s32 = a.s32;
+  s.groups = g.y, s.w32 = a.w32, s.s32 = a.s32, s.scale = q->scale, s.scale_host = q->scale_host;
   s.out[SET_PRE_W] = dpre_w, s.out[SET_PRE_B] = dpre_b, s.out[SET_POST_W] = dpost_w, s.out[SET_POST_B] = dpost_b;
   s.out[SET_GATE] = g.by_unit ? nullptr : dgate;
   if (!dpre_w && !dpre_b && !dpost_w && !dpost_b && !s.out[SET_GATE] && !dscale) return DM_OK;
-  const dim3 grid(dm_ceil_div(q->width, 64) + 1, SET_GATE + g.y);
-  if (dt == ACT8_F32) block_norm_sum_kernel<ACT8_F32><<<grid, 256, 0, st>>>(s);
-  else if (dt == ACT8_BF16) block_norm_sum_kernel<ACT8_BF16><<<grid, 256, 0, st>>>(s);
-  else block_norm_sum_kernel<ACT8_F16><<<grid, 256, 0, st>>>(s);
+  const dim3 grid(dm_ceil_div(q->width, 32) + 1, SET_GATE + g.y);
+  if (dt == ACT8_F32) block_norm_sum_kernel<ACT8_F32><<<grid, 1024, 0, st>>>(s);
+  else if (dt == ACT8_BF16) block_norm_sum_kernel<ACT8_BF16><<<grid, 1024, 0, st>>>(s);
+  else block_norm_sum_kernel<ACT8_F16><<<grid, 1024, 0, st>>>(s);
   DM_CHECK_LAUNCH();
   return DM_OK;
 }
