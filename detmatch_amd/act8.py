@@ -39,30 +39,56 @@ class Act8(object):
         return self.exps.to(torch.int32) - 127
 
 
+class _Stay(object):
+    """with _on(device) where the device is the current one already."""
+    __slots__ = ()
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_STAY = _Stay()
+
+
+def _on(dev):
+    """A context with `dev` as the current device (launches and streams go by the current device)."""
+    return _STAY if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
+
+
 def _device_of(*tensors):
     """The device that all tensors (or None) are on; raises unless it is one HIP device."""
     dev = None
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
-            raise _lib.DetMatchHipError('detmatch_amd ops run on the MI355X only (got a %s tensor); there is no CPU path'
-                                        % t.device)
-        if dev is not None and t.device != dev:
+        if dev is None:
+            if not t.is_cuda:
+                raise _lib.DetMatchHipError('detmatch_amd ops run on the MI355X only (got a %s tensor); there is no CPU path'
+                                            % t.device)
+            dev = t.device
+        elif t.device != dev:
+            if not t.is_cuda:
+                raise _lib.DetMatchHipError('detmatch_amd ops run on the MI355X only (got a %s tensor); there is no CPU path'
+                                            % t.device)
             raise ValueError('tensors on two devices: %s and %s' % (dev, t.device))
-        dev = t.device
     return dev
 
 
 def _dtype_code(t, what):
-    if t.dtype not in DTYPES:
+    code = DTYPES.get(t.dtype)
+    if code is None:
         raise TypeError('%s is %s: float32, bfloat16 or float16 is wanted' % (what, t.dtype))
-    return DTYPES[t.dtype]
+    return code
 
 
 def rows_view(x):
     """x (..., C) as (rows, C) with unit stride along C and non-overlapping rows (a copy where it has neither)."""
-    r = x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x
+    r = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    if r.is_contiguous():
+        return r
     if (r.shape[1] > 1 and r.stride(1) != 1) or (r.shape[0] > 1 and r.stride(0) < r.shape[1]):
         r = r.contiguous()
     return r
@@ -79,8 +105,8 @@ def pack(x):
         raise ValueError('pack needs at least one channel, got shape %s' % (tuple(x.shape),))
     code = _dtype_code(x, 'x')
     dev = _device_of(x)
-    with torch.cuda.device(dev):
-        r = rows_view(x.detach())
+    with _on(dev):
+        r = rows_view(x.detach() if x.requires_grad else x)
         rows, width = r.shape
         groups = (width + GROUP - 1) // GROUP
         codes = torch.empty((rows, groups * GROUP), dtype=torch.uint8, device=dev)
@@ -97,7 +123,7 @@ def unpack(kept, dtype=None):
         raise TypeError('unpack takes what pack returned, got %s' % type(kept).__name__)
     out = torch.empty(kept.shape, dtype=kept.dtype if dtype is None else dtype, device=kept.codes.device)
     code = _dtype_code(out, 'dtype')
-    with torch.cuda.device(_device_of(kept.codes, kept.exps)):
+    with _on(_device_of(kept.codes, kept.exps)):
         _lib.check(_lib.lib().dm_act8_unpack(_lib.ptr(kept.codes), _lib.ptr(kept.exps), kept.codes.shape[0], kept.shape[-1],
                                              _lib.ptr(out), code, _lib.stream()), 'dm_act8_unpack')
     return out
@@ -136,24 +162,30 @@ def _gemm(form, code, a, b, exps, bias, relu, m, n, k, out, bits=None, rowsum=No
     return out
 
 
+def _linear_forward(x, w, b, relu, keep, bits):
+    """y, and of x (rows, in) what `keep` asks for (an Act8 or None); bits: write the sign bits of y (or None)."""
+    code = DTYPES[x.dtype]
+    m, k = x.shape
+    n = w.shape[0]
+    y = torch.empty((m, n), dtype=x.dtype, device=x.device)
+    kept = pack(x) if keep else None
+    if m:
+        _gemm(0, code, _operand(rows_view(x), code), _operand(rows_view(w), code), None, None if b is None else b.contiguous(), relu, m, n, k,
+              y, bits)
+    return y, kept
+
+
 class _Linear8(Function):
 
     @staticmethod
-    def forward(ctx, x, w, b, relu, grad):
-        # (grad: is autograd recording; inside of a Function it never is)
-        code = DTYPES[x.dtype]
-        m, k = x.shape
-        n = w.shape[0]
-        needs = ctx.needs_input_grad if grad else (False,) * 3
-        with torch.cuda.device(x.device):
-            y = torch.empty((m, n), dtype=x.dtype, device=x.device)
-            bits = torch.empty((m, (n + 31) // 32), dtype=torch.int32, device=x.device) if relu and any(needs[:3]) else None
-            kept = pack(x) if needs[1] else None
-            if m:
-                _gemm(0, code, _operand(rows_view(x.detach()), code), _operand(rows_view(w.detach()), code), None,
-                      None if b is None else b.detach().contiguous(), relu, m, n, k, y, bits)
-        ctx.save_for_backward(w if needs[0] else None, kept.codes if kept else None, kept.exps if kept else None, bits)
-        ctx.sizes = (m, n, k)
+    def forward(ctx, x, w, b, relu):
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        m, n = x.shape[0], w.shape[0]
+        with _on(x.device):
+            bits = torch.empty((m, (n + 31) // 32), dtype=torch.int32, device=x.device) if relu else None
+            y, kept = _linear_forward(x, w, b, relu, need_w, bits)
+        ctx.save_for_backward(w if need_x else None, kept.codes if kept else None, kept.exps if kept else None, bits)
+        ctx.sizes = (m, n, x.shape[1])
         return y
 
     @staticmethod
@@ -162,27 +194,26 @@ class _Linear8(Function):
         w, codes, exps, bits = ctx.saved_tensors
         m, n, k = ctx.sizes
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        code = DTYPES[gy.dtype]
+        code, dtype, dev = DTYPES[gy.dtype], gy.dtype, gy.device
         gx = gw = gb = None
-        with torch.cuda.device(gy.device):
+        with _on(dev):
             if m == 0:
                 return (gy.new_zeros((0, k)) if need_x else None, gy.new_zeros((n, k)) if need_w else None,
-                        gy.new_zeros(n) if need_b else None, None, None)
+                        gy.new_zeros(n) if need_b else None, None)
             g = rows_view(gy)
             g = _operand(g, code) if bits is None else _masked(g, bits, code)
             if need_x:
-                gx = _gemm(1, code, g, _operand(rows_view(w.detach()), code), None, None, False, m, k, n,
-                           torch.empty((m, k), dtype=gy.dtype, device=gy.device))
+                gx = _gemm(1, code, g, _operand(rows_view(w), code), None, None, False, m, k, n, torch.empty((m, k), dtype=dtype, device=dev))
             if need_w or need_b:
-                gb = torch.empty(n, dtype=gy.dtype, device=gy.device) if need_b else None
+                gb = torch.empty(n, dtype=dtype, device=dev) if need_b else None
                 if need_w:
-                    gw = torch.empty((n, k), dtype=gy.dtype, device=gy.device)
-                    _gemm(2, code, g, (codes, codes.shape[1]), exps, None, False, n, k, m, gw, rowsum=gb)
+                    gw = _gemm(2, code, g, (codes, codes.shape[1]), exps, None, False, n, k, m,
+                               torch.empty((n, k), dtype=dtype, device=dev), rowsum=gb)
                 else:                         # a bias alone: its sums ride on a product with one group of zeros
-                    zero = torch.zeros((m, GROUP + 1), dtype=torch.uint8, device=gy.device)
-                    _gemm(2, code, g, (zero[:, :GROUP].contiguous(), GROUP), zero[:, GROUP:].contiguous(), None, False, n, GROUP, m,
-                          torch.empty((n, GROUP), dtype=gy.dtype, device=gy.device), rowsum=gb)
-        return gx, gw, gb, None, None
+                    zero = torch.zeros((2, m, GROUP), dtype=torch.uint8, device=dev)
+                    _gemm(2, code, g, (zero[0], GROUP), zero[1], None, False, n, GROUP, m,
+                          torch.empty((n, GROUP), dtype=dtype, device=dev), rowsum=gb)
+        return gx, gw, gb, None
 
 
 def linear(x, w, b=None, relu=False):
@@ -202,7 +233,12 @@ def linear(x, w, b=None, relu=False):
         if t is not None and t.dtype != x.dtype:
             raise TypeError('%s is %s, x is %s: one type is wanted' % (name, t.dtype, x.dtype))
     _device_of(x, w, b)
-    x2 = x.reshape(-1, x.shape[-1])
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     if max(x2.shape[0], w.shape[0], w.shape[1]) > _MAX:
         raise ValueError('sizes up to %d are wanted, got x %s, w %s' % (_MAX, tuple(x.shape), tuple(w.shape)))
-    return _Linear8.apply(x2, w, b, bool(relu), torch.is_grad_enabled()).view(*x.shape[:-1], w.shape[0])
+    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or (b is not None and b.requires_grad)):
+        y = _Linear8.apply(x2, w, b, bool(relu))
+    else:
+        with _on(x.device):
+            y, _ = _linear_forward(x2, w, b, bool(relu), False, None)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], w.shape[0])

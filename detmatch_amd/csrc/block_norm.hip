@@ -166,7 +166,7 @@ __device__ __forceinline__ void row_stats(const BnArgs &a, const float (&v)[NCH]
 
 // A workgroup's teams walk the rows with the grid's stride.  The next row's operands are under way while this one is computed.
 template <int T, bool LAYER, int NCH, int BLOCK>
-__global__ __launch_bounds__(BLOCK) void block_norm_fwd_kernel(BnArgs a) {
+__global__ __launch_bounds__(BLOCK, NCH == 1 ? 4 : 2) void block_norm_fwd_kernel(BnArgs a) {
   __shared__ float red[64];
   const int tx = threadIdx.x & (a.T - 1), team = threadIdx.x / a.T, teams = BLOCK / a.T, groups8 = (a.C + 31) / 32;
   int turn = 0;
