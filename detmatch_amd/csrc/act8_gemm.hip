@@ -10,6 +10,8 @@
 // lane ends with 4 neighbouring elements of a row of C.  Few output tiles and a long contraction: the contraction is split over
 // workgroups, partial sums go to a workspace and are added in split order by a second kernel (no atomics: the result is a
 // function of the shapes and values alone).
+#include <type_traits>
+
 #include "act8_codec.h"
 
 namespace {
@@ -22,8 +24,6 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-
-__device__ __attribute__((aligned(16))) const uint32_t a8_zeros[4] = {0, 0, 0, 0};   // source of what lies outside of an operand
 
 struct A8Args {
   const void *A, *B, *bias;
@@ -108,31 +108,62 @@ __device__ __forceinline__ void split3(float a, float b, uint32_t *p) {
 }
 
 // ---- tile staging ------------------------------------------------------------------------------------------------------
-typedef const __attribute__((address_space(1))) void *gptr_t;
 typedef __attribute__((address_space(3))) void *lptr_t;
 
-// 16-bit operand, 16-byte pieces straight from memory into LDS.  A wave's 64 pieces land side by side; the swizzle is in the
-// address that each lane reads.  Rows behind the operand repeat its last one (their results are not stored); the contraction
-// behind its end is 0.  (Rows are readable, and 0 along the contraction, up to the next multiple of 8 elements: the entry's contract.)
-template <int ROWS, int BK, int THREADS>
-__device__ __forceinline__ void stage_kc(uint16_t *S, const uint16_t *P, long long ld, int rows, int k0, int k_hi, int tid) {
-#pragma unroll
-  for (int h = 0; h < ROWS * BK / 8 / THREADS; ++h) {
-    const int i = tid + THREADS * h, row = i / (BK / 8), c = (i % (BK / 8)) ^ kc_swizzle<BK>(row), k = k0 + 8 * c;
-    const uint16_t *src = k < k_hi ? P + (long long)min(row, rows - 1) * ld + k : (const uint16_t *)a8_zeros;
-    __builtin_amdgcn_global_load_lds((gptr_t)src, (lptr_t)(S + (size_t)(i - (tid & 63)) * 8), 16, 0, 0);
-  }
-}
+// 16-bit operand, 16-byte pieces straight from memory into LDS, one BK after the other.  A wave's 64 pieces land side by side; the swizzle is
+// in the offset that each lane reads at.  What lies beside the operand (rows of a contraction-contiguous tile, columns of the other kind)
+// repeats its last part, and its results are not stored; the contraction behind its end is 0.  (Rows are readable, and 0 along the
+// contraction, up to the next multiple of 8 elements: the entry's contract.)  A whole step is exactly H loads.
+// Buffer loads: a tile's base is uniform, a lane's offset in it (< 2^31 bytes, checked by the entry) the same in every step.  (The global form of
+// these loads makes the compiler wait for all LDS reads under way before each matrix instruction.)
+constexpr int BUFFER_WORD3 = 0x00027000;         // untyped 32-bit data
 
-template <int COLS, int BK, int THREADS>
-__device__ __forceinline__ void stage_kr(uint16_t *S, const uint16_t *P, long long ld, int cols, int k0, int k_hi, int tid) {
+template <bool ALONG_K, int SIDE, int BK, int THREADS>
+struct Stager {
+  static constexpr int H = SIDE * BK / 8 / THREADS;
+  const uint16_t *base;
+  long long step;                // elements from one step's tile to the next
+  uint32_t at[H];                // bytes from the base
+  int k[H];                      // where piece h lies along the contraction, from the step's begin on
+
+  __device__ __forceinline__ void start(const uint16_t *P, long long ld, int side0, int side, int k0, int tid) {
+    base = P + (ALONG_K ? k0 * ld + side0 : side0 * ld + k0);
+    step = ALONG_K ? BK * ld : BK;
 #pragma unroll
-  for (int h = 0; h < COLS * BK / 8 / THREADS; ++h) {
-    const int i = tid + THREADS * h, r = i / (COLS / 8), c = (i % (COLS / 8)) ^ kr_swizzle(r), k = k0 + r;
-    const uint16_t *src = k < k_hi ? P + (long long)k * ld + min(8 * c, ((cols + 7) & ~7) - 8) : (const uint16_t *)a8_zeros;
-    __builtin_amdgcn_global_load_lds((gptr_t)src, (lptr_t)(S + (size_t)(i - (tid & 63)) * 8), 16, 0, 0);
+    for (int h = 0; h < H; ++h) {
+      const int i = tid + THREADS * h;
+      if (!ALONG_K) {
+        const int row = i / (BK / 8);
+        k[h] = 8 * ((i % (BK / 8)) ^ kc_swizzle<BK>(row));
+        at[h] = 2 * ((uint32_t)min(row, side - 1 - side0) * (uint32_t)ld + k[h]);
+      } else {
+        k[h] = i / (SIDE / 8);
+        const int c = (i % (SIDE / 8)) ^ kr_swizzle(k[h]);
+        at[h] = 2 * ((uint32_t)k[h] * (uint32_t)ld + min(8 * c, ((side - side0 + 7) & ~7) - 8));
+      }
+    }
   }
-}
+
+  // left: what is left of the contraction at this step's begin
+  __device__ __forceinline__ void issue(uint16_t *S, int wave, int left) {
+#ifdef __HIP_DEVICE_COMPILE__                       // (the host pass has no type for a buffer descriptor)
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, 0x7fffffff, BUFFER_WORD3);
+    base += step;
+    if (left >= BK) {
+#pragma unroll
+      for (int h = 0; h < H; ++h)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lptr_t)(S + (size_t)(wave * 64 + THREADS * h) * 8), 16, at[h], 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        uint16_t *d = S + (size_t)(wave * 64 + THREADS * h) * 8;
+        if (k[h] < left) __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lptr_t)d, 16, at[h], 0, 0, 0);
+        else *(uint4 *)(d + 8 * (threadIdx.x & 63)) = make_uint4(0, 0, 0, 0);
+      }
+    }
+#endif
+  }
+};
 
 // 8-bit operand: 16 codes of a row at a time through registers
 template <int COLS, int BK, int THREADS>
@@ -261,130 +292,234 @@ __device__ __forceinline__ void put4(const A8Args &a, int m, int n, const float 
   }
 }
 
-// one 32 x 32 block: lane -> row m0 + (lane & 31), columns n0 + 8 q + 4 (lane >> 5) + 0..3 for q = 0..3
+// 32 rows x 64 columns of a wave's results, from row m0 and column n0 on.  They go through LDS, 32 x 68 floats of the wave's own, so that
+// 8 lanes write 64 neighbouring elements of a row: straight from the accumulators an instruction would write 16 bytes in each of 32 rows
+// (4 096 x 4 096 bf16 results of a product over 64: 46 us, this way 14).
+constexpr int EPI_PITCH = 68, EPI_FLOATS = 32 * EPI_PITCH;
+
 template <int T>
-__device__ __forceinline__ void store_block(const A8Args &a, const Tile &t, const f32x16 &acc, int m0, int n0, int lane) {
-  const int m = m0 + (lane & 31);
-  uint32_t word = 0;
+__device__ __forceinline__ void store_rows(const A8Args &a, const Tile &t, const f32x16 &left, const f32x16 &right, float *S, const float *bias,
+                                           int m0, int n0, int lane) {
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    const int n = n0 + 8 * q + 4 * (lane >> 5);
-    float v[4] = {acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+    float *d = S + (lane & 31) * EPI_PITCH + 8 * q + 4 * (lane >> 5);
+    *(float4 *)d = make_float4(left[4 * q], left[4 * q + 1], left[4 * q + 2], left[4 * q + 3]);
+    *(float4 *)(d + 32) = make_float4(right[4 * q], right[4 * q + 1], right[4 * q + 2], right[4 * q + 3]);
+  }
+  __builtin_amdgcn_wave_barrier();
+  const int n = n0 + 8 * (lane & 7);
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int m = m0 + 8 * r + (lane >> 3);
+    const float *p = S + (8 * r + (lane >> 3)) * EPI_PITCH + 8 * (lane & 7);
+    const float4 lo = *(const float4 *)p, hi = *(const float4 *)(p + 4);
+    float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    const int left_n = m < a.M ? a.N - n : 0;
     if (a.splits > 1) {
-      float *p = a.part + ((size_t)t.split * a.M + m) * a.N + n;
-      if (m < a.M) {
-        if (a.N % 4 == 0 && n + 3 < a.N) *(float4 *)p = make_float4(v[0], v[1], v[2], v[3]);
-        else
-          for (int k = 0; k < 4; ++k)
-            if (n + k < a.N) p[k] = v[k];
-      }
+      act8_store8<ACT8_F32>(a.part, ((size_t)t.split * a.M + m) * a.N + n, left_n, v);
       continue;
     }
-    finish4<T>(a, m, n, v);
+    uint32_t word = 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (v[k] > 0.f) word |= 1u << (8 * q + 4 * (lane >> 5) + k);
+    for (int k = 0; k < 8; ++k) {
+      v[k] += bias[k];
+      if (v[k] > 0.f) word |= 1u << k;
       if (a.relu) v[k] = v[k] < 0.f ? 0.f : v[k];            // (a nan stays one)
     }
-    if (m < a.M) put4<T>(a, m, n, v);
+    act8_store8<T>(a.C, (size_t)m * a.N + n, left_n, v);
+    if (a.bits) {
+      word <<= 8 * (lane & 3);
+      word |= __shfl_xor(word, 1), word |= __shfl_xor(word, 2);
+      if ((lane & 3) == 0 && left_n > 0) a.bits[(size_t)m * ((a.N + 31) / 32) + n / 32] = word;
+    }
   }
-  if (a.bits && a.splits == 1) {
-    word |= __shfl_xor(word, 32);
-    if (lane < 32 && m < a.M && n0 < a.N) a.bits[(size_t)m * ((a.N + 31) / 32) + n0 / 32] = word;
-  }
+  __builtin_amdgcn_wave_barrier();
+}
+
+// the bias of the 8 columns that a lane writes
+template <int T>
+__device__ __forceinline__ void load_bias(const A8Args &a, int n0, int lane, float *v) {
+  const int n = n0 + 8 * (lane & 7);
+  if (a.bias && a.splits == 1) act8_load8<T>(a.bias, n, a.N - n, v);
+  else
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = 0.f;
 }
 
 // ---- the 16-bit product --------------------------------------------------------------------------------------------------
-template <int T, int FORM, int WM, int WN, int FM, int FN>
-__global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 ? 2 : 1) void a8_gemm16_kernel(A8Args a) {
-  constexpr int BM = WM * FM * 32, BN = WN * FN * 32, BK = 64, THREADS = 64 * WM * WN;
-  extern __shared__ __attribute__((aligned(16))) uint16_t a8_lds[];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / WN, wn = wave % WN;
+// STAGES tiles of BK in LDS.  Fragments are read one group of 16 of the contraction ahead of the matrix instructions, also across the border of
+// two steps: before a step's last group is multiplied, the wave waits for its own loads of the next step (all but those issued after
+// them) and for its last fragments, and meets the others at the barrier.  Behind it the next tile is complete, and nobody reads this step's
+// any more: the loads of step s + STAGES go there.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (15 << 8) | (7 << 4));       // vmcnt(N)
+}
+
+// (Builtins and not inline assembly: the compiler then knows that no scalar load is pending either, and waits for the fragments that it
+// needs instead of for all that are under way.)
+__device__ __forceinline__ void meet() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4));                                 // lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+template <int T>
+__device__ __forceinline__ float add8(s16x8 v, float acc) {          // acc + the sum of 8 values
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if constexpr (T == ACT8_F16) {
+      const f16x2 x = {__builtin_bit_cast(f16x8, v)[2 * k], __builtin_bit_cast(f16x8, v)[2 * k + 1]}, one = {(_Float16)1.f, (_Float16)1.f};
+      acc = __builtin_amdgcn_fdot2(x, one, acc, false);
+    } else {
+      const __bf16 b1 = (__bf16)1.f;
+      const bf16x2 x = {__builtin_bit_cast(bf16x8, v)[2 * k], __builtin_bit_cast(bf16x8, v)[2 * k + 1]}, one = {b1, b1};
+      acc = __builtin_amdgcn_fdot2_f32_bf16(x, one, acc, false);
+    }
+  }
+  return acc;
+}
+
+// row sums (form 2): lane -> column m0 + (lane & 31) of A, half of the contraction each
+template <int T>
+__device__ __forceinline__ void store_sum(const A8Args &a, const Tile &t, float v, int m0, int lane) {
+  v += __shfl_xor(v, 32);
+  const int m = m0 + lane;
+  if (lane >= 32 || m >= a.M) return;
+  if (a.splits > 1) a.part[(size_t)a.splits * a.M * a.N + (size_t)t.split * a.M + m] = v;
+  else act8_put<T>(a.rowsum, m, v);
+}
+
+template <int T, int FORM, int WM, int WN, int FM, int FN, int BK, int STAGES>
+__global__ __launch_bounds__(64 * WM * WN, 2) void a8_gemm16_kernel(A8Args a) {
+  constexpr int BM = WM * FM * 32, BN = WN * FN * 32, THREADS = 64 * WM * WN, STAGE = (BM + BN) * BK;
+  extern __shared__ __attribute__((aligned(16))) uint16_t a8_lds[];      // [STAGES][A tile, B tile]
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
   Tile t;
   if (!tile_of(a, &t)) return;
   const int m0 = t.m * BM, n0 = t.n * BN;
   const int s_lo = t.split * a.steps_per_split, s_hi = min((a.K + BK - 1) / BK, s_lo + a.steps_per_split);
-  const uint16_t *A = (const uint16_t *)a.A + (FORM == 2 ? (long long)m0 : (long long)m0 * a.lda);
-  const uint16_t *B = (const uint16_t *)a.B + (FORM == 1 ? (long long)n0 : (long long)n0 * a.ldb);      // (form 2: unused)
-  const bool sums = FORM == 2 && a.rowsum && t.n == 0 && wn == 0;
-  f32x16 acc[FM][FN], sum[FORM == 2 ? FM : 1];
+  f32x16 acc[FM][FN];
+  float sum[FM];
 #pragma unroll
-  for (int i = 0; i < FM; ++i)
+  for (int i = 0; i < FM; ++i) {
+    sum[i] = 0.f;
 #pragma unroll
     for (int j = 0; j < FN; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-#pragma unroll
-  for (int i = 0; i < (FORM == 2 ? FM : 1); ++i)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) sum[i][r] = 0.f;
-  const short one = T == ACT8_F16 ? 0x3c00 : 0x3f80;
-  const s16x8 ones = {one, one, one, one, one, one, one, one};
+  }
+  typedef Stager<FORM == 2, BM, BK, THREADS> SA;
+  typedef Stager<FORM == 1, BN, BK, THREADS> SB;
+  SA sa;
+  SB sb;
   CodeRegs<BN, BK, THREADS> codes;
+  constexpr int LOADS = SA::H + (FORM == 2 ? 0 : SB::H);
+  sa.start((const uint16_t *)a.A, a.lda, m0, a.M, s_lo * BK, tid);
+  if constexpr (FORM != 2) sb.start((const uint16_t *)a.B, a.ldb, n0, a.N, s_lo * BK, tid);
 
-  auto stage = [&](int s, int buf) {
-    const int k0 = s * BK;
-    if constexpr (FORM == 2) {
-      stage_kr<BM, BK, THREADS>((a8_lds + buf * BM * BK), A, a.lda, a.M - m0, k0, a.K, tid);
-      fetch_codes<BN, BK, THREADS>(codes, (const uint8_t *)a.B, a.exps, a.ldb, n0, k0, a.K, tid);
-    } else {
-      stage_kc<BM, BK, THREADS>((a8_lds + buf * BM * BK), A, a.lda, a.M - m0, k0, a.K, tid);
-      if constexpr (FORM == 0) stage_kc<BN, BK, THREADS>((a8_lds + 2 * BM * BK + buf * BN * BK), B, a.ldb, a.N - n0, k0, a.K, tid);
-      else stage_kr<BN, BK, THREADS>((a8_lds + 2 * BM * BK + buf * BN * BK), B, a.ldb, a.N - n0, k0, a.K, tid);
-    }
+  auto fetch = [&](int s) {
+    if constexpr (FORM == 2) fetch_codes<BN, BK, THREADS>(codes, (const uint8_t *)a.B, a.exps, a.ldb, n0, s * BK, a.K, tid);
+  };
+  auto issue = [&](int s, int buf) {
+    sa.issue(a8_lds + buf * STAGE, wave, a.K - s * BK);
+    if constexpr (FORM != 2) sb.issue(a8_lds + buf * STAGE + BM * BK, wave, a.K - s * BK);
+  };
+  auto put_codes = [&](int buf) {
+    if constexpr (FORM == 2) store_codes<T, BN, BK, THREADS>(codes, a8_lds + buf * STAGE + BM * BK, tid);
   };
 
-  if (s_lo < s_hi) {
-    stage(s_lo, 0);
-    if constexpr (FORM == 2) store_codes<T, BN, BK, THREADS>(codes, a8_lds + 2 * BM * BK, tid);
+  const int steps = s_hi - s_lo;
+#pragma unroll
+  for (int i = 0; i < STAGES; ++i) {
+    if (i < steps) {
+      fetch(s_lo + i);
+      issue(s_lo + i, i);
+      if (i < STAGES - 1) put_codes(i);                    // (the last ones wait in registers)
+    }
   }
-  for (int s = s_lo; s < s_hi; ++s) {
-    const int buf = (s - s_lo) & 1;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // this step's tiles have landed ...
-    __syncthreads();                                      // ... for all waves, and nobody reads the other pair any more
-    if (s + 1 < s_hi) stage(s + 1, buf ^ 1);
+  s16x8 fa[2][FM], fb[2][FN];
+  auto read = [&](int buf, int kk) {
+    const uint16_t *As = a8_lds + buf * STAGE, *Bs = As + BM * BK;
 #pragma unroll
-    for (int kk = 0; kk < BK / 16; ++kk) {
-      s16x8 fa[FM], fb[FN];
+    for (int i = 0; i < FM; ++i) {
+      if constexpr (FORM == 2) fa[kk & 1][i] = frag_kr<BM>(As, (wm * FM + i) * 32, kk, lane);
+      else fa[kk & 1][i] = frag_kc<BK>(As, (wm * FM + i) * 32, kk, lane);
+    }
 #pragma unroll
-      for (int i = 0; i < FM; ++i) {
-        if constexpr (FORM == 2) fa[i] = frag_kr<BM>((a8_lds + buf * BM * BK), (wm * FM + i) * 32, kk, lane);
-        else fa[i] = frag_kc<BK>((a8_lds + buf * BM * BK), (wm * FM + i) * 32, kk, lane);
-      }
-#pragma unroll
-      for (int j = 0; j < FN; ++j) {
-        if constexpr (FORM == 0) fb[j] = frag_kc<BK>((a8_lds + 2 * BM * BK + buf * BN * BK), (wn * FN + j) * 32, kk, lane);
-        else fb[j] = frag_kr<BN>((a8_lds + 2 * BM * BK + buf * BN * BK), (wn * FN + j) * 32, kk, lane);
-      }
+    for (int j = 0; j < FN; ++j) {
+      if constexpr (FORM == 0) fb[kk & 1][j] = frag_kc<BK>(Bs, (wn * FN + j) * 32, kk, lane);
+      else fb[kk & 1][j] = frag_kr<BN>(Bs, (wn * FN + j) * 32, kk, lane);
+    }
+  };
+  if (steps > 0) {
+    if (steps > STAGES) wait_loads<LOADS * (STAGES - 1)>();    // (the very last step may be less than LOADS)
+    else wait_loads<0>();
+    meet();
+    read(0, 0);
+  }
+  auto loop = [&](auto with_sums) {                        // (one branch outside of the loop: a branch inside keeps instructions from mixing)
+    auto multiply = [&](int kk) {
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < FM; ++i)
 #pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = mfma16<T>(fb[j], fa[i], acc[i][j]);
-      if constexpr (FORM == 2) {
-        if (sums) {
+        for (int j = 0; j < FN; ++j) acc[i][j] = mfma16<T>(fb[kk & 1][j], fa[kk & 1][i], acc[i][j]);
+      if constexpr (decltype(with_sums)::value) {
 #pragma unroll
-          for (int i = 0; i < FM; ++i) sum[i] = mfma16<T>(ones, fa[i], sum[i]);
-        }
+        for (int i = 0; i < FM; ++i) sum[i] = add8<T>(fa[kk & 1][i], sum[i]);
       }
-    }
-    if constexpr (FORM == 2) {
-      if (s + 1 < s_hi) store_codes<T, BN, BK, THREADS>(codes, a8_lds + 2 * BM * BK + (buf ^ 1) * BN * BK, tid);
-    }
-  }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    int buf = 0, s = 0;
+    // steps with STAGES more behind them, without a branch
+    for (; s + STAGES < steps; ++s) {
 #pragma unroll
-  for (int i = 0; i < FM; ++i)
+      for (int kk = 0; kk + 1 < BK / 16; ++kk) {
+        read(buf, kk + 1);
+        multiply(kk);
+      }
+      const int now = buf, before = now == 0 ? STAGES - 1 : now - 1;
+      buf = buf + 1 == STAGES ? 0 : buf + 1;
+      put_codes(before);              // what arrived during this step belongs to step s + STAGES - 1, in the buffer of the step before this one
+      wait_loads<LOADS * (STAGES - 2)>();
+      meet();
+      read(buf, 0);
+      fetch(s_lo + s + STAGES);
+      issue(s_lo + s + STAGES, now);
+      multiply(BK / 16 - 1);
+    }
+    for (; s < steps; ++s) {
 #pragma unroll
-    for (int j = 0; j < FN; ++j) store_block<T>(a, t, acc[i][j], m0 + (wm * FM + i) * 32, n0 + (wn * FN + j) * 32, lane);
+      for (int kk = 0; kk + 1 < BK / 16; ++kk) {
+        read(buf, kk + 1);
+        multiply(kk);
+      }
+      if (s + 1 < steps) {
+        const int before = buf == 0 ? STAGES - 1 : buf - 1;
+        buf = buf + 1 == STAGES ? 0 : buf + 1;
+        if (s + STAGES == steps) put_codes(before);
+        wait_loads<0>();              // (fewer loads behind the next step's than in the middle: wait for all)
+        meet();
+        read(buf, 0);
+      }
+      multiply(BK / 16 - 1);
+    }
+  };
+  const bool sums = FORM == 2 && a.rowsum && t.n == 0 && wn == 0;
   if constexpr (FORM == 2) {
-    if (sums && lane < 32) {
+    if (sums) loop(std::true_type{});
+    else loop(std::false_type{});
+  } else loop(std::false_type{});
+  static_assert(FN == 2, "store_rows takes two blocks side by side");
+  __syncthreads();                                         // the tiles have been read: their place is free
+  float bias[8];
+  load_bias<T>(a, n0 + wn * 64, lane, bias);
 #pragma unroll
-      for (int i = 0; i < FM; ++i) {
-        const int m = m0 + (wm * FM + i) * 32 + lane;
-        if (m >= a.M) continue;
-        if (a.splits > 1) a.part[(size_t)a.splits * a.M * a.N + (size_t)t.split * a.M + m] = sum[i][0];
-        else act8_put<T>(a.rowsum, m, sum[i][0]);
-      }
-    }
+  for (int i = 0; i < FM; ++i) {
+    store_rows<T>(a, t, acc[i][0], acc[i][1], (float *)a8_lds + wave * EPI_FLOATS, bias, m0 + (wm * FM + i) * 32, n0 + wn * 64, lane);
+    if (FORM == 2 && sums) store_sum<T>(a, t, sum[i], m0 + (wm * FM + i) * 32, lane);
   }
 }
 
@@ -402,17 +537,16 @@ __global__ __launch_bounds__(256) void a8_gemm32_kernel(A8Args a) {
   const int m0 = t.m * BM, n0 = t.n * BN;
   const int s_lo = t.split * a.steps_per_split, s_hi = min((a.K + BK - 1) / BK, s_lo + a.steps_per_split);
   const bool sums = FORM == 2 && a.rowsum && t.n == 0 && wn == 0;
-  f32x16 acc[FM][FN], sum[FM];
+  f32x16 acc[FM][FN];
+  float sum[FM];
 #pragma unroll
-  for (int i = 0; i < FM; ++i)
+  for (int i = 0; i < FM; ++i) {
+    sum[i] = 0.f;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      sum[i][r] = 0.f;
+    for (int j = 0; j < FN; ++j)
 #pragma unroll
-      for (int j = 0; j < FN; ++j) acc[i][j][r] = 0.f;
-    }
-  const short one = 0x3f80;
-  const s16x8 ones = {one, one, one, one, one, one, one, one};
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+  }
   F32Regs<BM, BK, THREADS> ra;
   F32Regs<BN, BK, THREADS> rb;
   CodeRegs<BN, BK, THREADS> codes;
@@ -464,25 +598,18 @@ __global__ __launch_bounds__(256) void a8_gemm32_kernel(A8Args a) {
 #pragma unroll
           for (int q = 2; q >= 0; --q)
 #pragma unroll
-            for (int i = 0; i < FM; ++i) sum[i] = mfma16<ACT8_BF16>(ones, fa[q][i], sum[i]);
+            for (int i = 0; i < FM; ++i) sum[i] = add8<ACT8_BF16>(fa[q][i], sum[i]);
         }
       }
     }
   }
+  __syncthreads();                                         // the tiles have been read: their place is free
+  float bias[8];
+  load_bias<ACT8_F32>(a, n0 + wn * 64, lane, bias);
 #pragma unroll
-  for (int i = 0; i < FM; ++i)
-#pragma unroll
-    for (int j = 0; j < FN; ++j) store_block<ACT8_F32>(a, t, acc[i][j], m0 + (wm * FM + i) * 32, n0 + (wn * FN + j) * 32, lane);
-  if constexpr (FORM == 2) {
-    if (sums && lane < 32) {
-#pragma unroll
-      for (int i = 0; i < FM; ++i) {
-        const int m = m0 + (wm * FM + i) * 32 + lane;
-        if (m >= a.M) continue;
-        if (a.splits > 1) a.part[(size_t)a.splits * a.M * a.N + (size_t)t.split * a.M + m] = sum[i][0];
-        else ((float *)a.rowsum)[m] = sum[i][0];
-      }
-    }
+  for (int i = 0; i < FM; ++i) {
+    store_rows<ACT8_F32>(a, t, acc[i][0], acc[i][1], (float *)a8_lds + wave * EPI_FLOATS, bias, m0 + (wm * FM + i) * 32, n0 + wn * 64, lane);
+    if (FORM == 2 && sums) store_sum<ACT8_F32>(a, t, sum[i], m0 + (wm * FM + i) * 32, lane);
   }
 }
 
@@ -549,19 +676,52 @@ __global__ __launch_bounds__(256) void a8_mask_kernel(const void *__restrict__ x
   }
 }
 
+#ifndef A8_BIG_TILES
+#define A8_BIG_TILES 200   // large tiles from so many of them on
+#endif
+#ifndef A8_SBK
+#define A8_SBK 64
+#endif
+#ifndef A8_SST
+#define A8_SST 2
+#endif
+#ifndef A8_BIG2
+#define A8_BIG2 2, 2, 4, 2, 32, 3
+#endif
+#ifndef A8_BIG0
+#define A8_BIG0 2, 4, 4, 2, 64, 2
+#endif
+
+template <int WM_, int WN_, int FM_, int FN_, int BK_, int STAGES_>
+struct Shape {
+  static constexpr int WM = WM_, WN = WN_, FM = FM_, FN = FN_, BK = BK_, STAGES = STAGES_, BM = WM * FM * 32, BN = WN * FN * 32,
+                       THREADS = 64 * WM * WN, LDS = STAGES * (BM + BN) * BK * 2;
+};
+typedef Shape<2, 2, 2, 2, A8_SBK, A8_SST> Small;
+typedef Shape<A8_BIG0> BigForward;      // forms 0 and 1
+typedef Shape<A8_BIG2> BigWeight;       // form 2
+
+constexpr long long A8_MAX_PITCH = (1ll << 31) / 512 - 8;
+
 struct Plan {
-  int bm, bn, bk, tiles_m, tiles_n, splits, steps_per_split;
+  int big, bm, bn, bk, tiles_m, tiles_n, splits, steps_per_split;
 };
 
-Plan a8_plan(int dtype, int M, int N, int K) {
+Plan a8_plan(int form, int dtype, int M, int N, int K) {
   Plan p;
   p.bm = p.bn = 128;
-  p.bk = dtype == ACT8_F32 ? 32 : 64;
+  p.bk = dtype == ACT8_F32 ? 32 : Small::BK;
+  p.big = 0;
+  if (dtype != ACT8_F32) {
+    const int bm = form == 2 ? BigWeight::BM : BigForward::BM, bn = form == 2 ? BigWeight::BN : BigForward::BN;
+    if ((long long)dm_ceil_div(M, bm) * dm_ceil_div(N, bn) >= A8_BIG_TILES)
+      p.big = 1, p.bm = bm, p.bn = bn, p.bk = form == 2 ? BigWeight::BK : BigForward::BK;
+  }
   p.tiles_m = dm_ceil_div(M, p.bm), p.tiles_n = dm_ceil_div(N, p.bn);
   const long long tiles = (long long)p.tiles_m * p.tiles_n;
   const int steps = dm_ceil_div(K, p.bk);
-  long long want = tiles >= 256 ? 1 : (512 + tiles - 1) / tiles;
-  const long long most = steps / 4;                                     // a split has 4 steps at least
+  long long want = p.big || tiles >= 256 ? 1 : (512 + tiles - 1) / tiles;
+  const long long most = (long long)steps * p.bk / 256;                 // a split has 256 of the contraction at least
   if (want > most) want = most;
   if (want > 64) want = 64;
   if (want < 1) want = 1;
@@ -570,18 +730,26 @@ Plan a8_plan(int dtype, int M, int N, int K) {
   return p;
 }
 
-template <int T, int FORM>
+template <int T, int FORM, typename S>
 int launch16(const A8Args &a, unsigned grid, hipStream_t st) {
-  auto k = a8_gemm16_kernel<T, FORM, 2, 2, 2, 2>;
-  const size_t lds = 2 * (128 + 128) * 64 * 2;
-  k<<<grid, 256, lds, st>>>(a);
+  auto k = a8_gemm16_kernel<T, FORM, S::WM, S::WN, S::FM, S::FN, S::BK, S::STAGES>;
+  if (S::LDS > 65536) DM_HIP(hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS));
+  k<<<grid, S::THREADS, S::LDS, st>>>(a);
   DM_CHECK_LAUNCH();
   return DM_OK;
 }
 
+template <int T>
+int launch16(int form, const A8Args &a, const Plan &p, unsigned grid, hipStream_t st) {
+  if (form == 0) return p.big ? launch16<T, 0, BigForward>(a, grid, st) : launch16<T, 0, Small>(a, grid, st);
+  if (form == 1) return p.big ? launch16<T, 1, BigForward>(a, grid, st) : launch16<T, 1, Small>(a, grid, st);
+  return p.big ? launch16<T, 2, BigWeight>(a, grid, st) : launch16<T, 2, Small>(a, grid, st);
+}
+
 template <int FORM>
 int launch32(const A8Args &a, unsigned grid, hipStream_t st) {
-  a8_gemm32_kernel<FORM><<<grid, 256, (size_t)(3 * 128 * 32 + (FORM == 2 ? 1 : 3) * 128 * 32) * 2, st>>>(a);
+  constexpr size_t tiles = (size_t)(3 * 128 * 32 + (FORM == 2 ? 1 : 3) * 128 * 32) * 2, rows = (size_t)4 * EPI_FLOATS * sizeof(float);
+  a8_gemm32_kernel<FORM><<<grid, 256, tiles > rows ? tiles : rows, st>>>(a);
   DM_CHECK_LAUNCH();
   return DM_OK;
 }
@@ -599,7 +767,7 @@ int reduce(const A8Args &a, hipStream_t st) {
 
 extern "C" size_t dm_act8_gemm_workspace_bytes(int form, int dtype, int M, int N, int K) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  const Plan p = a8_plan(dtype, M, N, K);
+  const Plan p = a8_plan(form, dtype, M, N, K);
   return p.splits > 1 ? dm_align(((size_t)p.splits * M * N + (form == 2 ? (size_t)p.splits * M : 0)) * sizeof(float)) : 0;
 }
 
@@ -614,10 +782,12 @@ extern "C" int dm_act8_gemm(int form, int dtype, const void *A, long long lda, c
   if (form == 2 && (ldb % 32 || ((uintptr_t)B & 15))) return DM_ERR_INVALID_ARG;
   A8Args a = {};
   if (dtype != ACT8_F32) {
-    // 16-byte pieces: no piece crosses a row's end (the pitch has room for the last one), every address is a multiple of 16
+    // 16-byte pieces: no piece crosses a row's end (the pitch has room for the last one), every address is a multiple of 16, and a tile's
+    // 256 rows are less than 2^31 bytes
+    if (lda > A8_MAX_PITCH || (form != 2 && ldb > A8_MAX_PITCH)) return DM_ERR_UNSUPPORTED;
     if (lda % 8 || ((uintptr_t)A & 15) || (form != 2 && (ldb % 8 || ((uintptr_t)B & 15)))) return DM_ERR_UNSUPPORTED;
   }
-  const Plan p = a8_plan(dtype, M, N, K);
+  const Plan p = a8_plan(form, dtype, M, N, K);
   a.A = A, a.B = B, a.bias = bias, a.exps = exps, a.C = C, a.bits = sign_bits, a.rowsum = rowsum;
   a.M = M, a.N = N, a.K = K, a.lda = lda, a.ldb = ldb, a.relu = relu;
   a.splits = p.splits, a.steps_per_split = p.steps_per_split, a.tiles_m = p.tiles_m, a.tiles_n = p.tiles_n;
@@ -632,10 +802,7 @@ extern "C" int dm_act8_gemm(int form, int dtype, const void *A, long long lda, c
   const unsigned grid = (unsigned)a.per_xcd * 8;
   int rc;
   if (dtype == ACT8_F32) rc = form == 0 ? launch32<0>(a, grid, st) : form == 1 ? launch32<1>(a, grid, st) : launch32<2>(a, grid, st);
-  else if (dtype == ACT8_BF16)
-    rc = form == 0 ? launch16<ACT8_BF16, 0>(a, grid, st) : form == 1 ? launch16<ACT8_BF16, 1>(a, grid, st) : launch16<ACT8_BF16, 2>(a, grid, st);
-  else
-    rc = form == 0 ? launch16<ACT8_F16, 0>(a, grid, st) : form == 1 ? launch16<ACT8_F16, 1>(a, grid, st) : launch16<ACT8_F16, 2>(a, grid, st);
+  else rc = dtype == ACT8_BF16 ? launch16<ACT8_BF16>(form, a, p, grid, st) : launch16<ACT8_F16>(form, a, p, grid, st);
   if (rc != DM_OK || p.splits == 1) return rc;
   return dtype == ACT8_F32 ? reduce<ACT8_F32>(a, st) : dtype == ACT8_BF16 ? reduce<ACT8_BF16>(a, st) : reduce<ACT8_F16>(a, st);
 }
