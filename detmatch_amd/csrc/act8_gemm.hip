@@ -266,15 +266,6 @@ __device__ __forceinline__ bool tile_of(const A8Args &a, Tile *t) {
 
 // 4 neighbouring elements of row m from n on
 template <int T>
-__device__ __forceinline__ void finish4(const A8Args &a, int m, int n, float *v) {
-  if (a.bias) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (n + k < a.N) v[k] += act8_get<T>(a.bias, n + k);
-  }
-}
-
-template <int T>
 __device__ __forceinline__ void put4(const A8Args &a, int m, int n, const float *v) {
   const size_t at = (size_t)m * a.N + n;
   if (a.vec_c && n + 3 < a.N) {
@@ -391,11 +382,13 @@ __device__ __forceinline__ void store_sum(const A8Args &a, const Tile &t, float 
   else act8_put<T>(a.rowsum, m, v);
 }
 
-template <int T, int FORM, int WM, int WN, int FM, int FN, int BK, int STAGES>
-__global__ __launch_bounds__(64 * WM * WN, 2) void a8_gemm16_kernel(A8Args a) {
-  constexpr int BM = WM * FM * 32, BN = WN * FN * 32, THREADS = 64 * WM * WN, STAGE = (BM + BN) * BK;
+// WK groups of WM x WN waves share a tile: each multiplies its part of every step's contraction, and they add up at the end.
+template <int T, int FORM, int WM, int WN, int FM, int FN, int BK, int STAGES, int WK>
+__global__ __launch_bounds__(64 * WM * WN * WK, 2) void a8_gemm16_kernel(A8Args a) {
+  constexpr int BM = WM * FM * 32, BN = WN * FN * 32, THREADS = 64 * WM * WN * WK, STAGE = (BM + BN) * BK;
   extern __shared__ __attribute__((aligned(16))) uint16_t a8_lds[];      // [STAGES][A tile, B tile]
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wk = wave / (WM * WN),
+            wm = wave % (WM * WN) / WN, wn = wave % WN;
   Tile t;
   if (!tile_of(a, &t)) return;
   const int m0 = t.m * BM, n0 = t.n * BN;
@@ -439,18 +432,22 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void a8_gemm16_kernel(A8Args a) {
       if (i < STAGES - 1) put_codes(i);                    // (the last ones wait in registers)
     }
   }
+  constexpr int KK = BK / 16 / WK;                         // groups of 16 that a wave multiplies of a step
+  static_assert(KK % 2 == 0, "a fragment set's index is a constant in the unrolled loops");
   s16x8 fa[2][FM], fb[2][FN];
-  auto read = [&](int buf, int kk) {
+  auto read = [&](int buf, int kk) {                       // kk == KK: the first of the tile in buf
+    const int set = kk % 2;
+    kk = wk * KK + kk % KK;
     const uint16_t *As = a8_lds + buf * STAGE, *Bs = As + BM * BK;
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
-      if constexpr (FORM == 2) fa[kk & 1][i] = frag_kr<BM>(As, (wm * FM + i) * 32, kk, lane);
-      else fa[kk & 1][i] = frag_kc<BK>(As, (wm * FM + i) * 32, kk, lane);
+      if constexpr (FORM == 2) fa[set][i] = frag_kr<BM>(As, (wm * FM + i) * 32, kk, lane);
+      else fa[set][i] = frag_kc<BK>(As, (wm * FM + i) * 32, kk, lane);
     }
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
-      if constexpr (FORM == 0) fb[kk & 1][j] = frag_kc<BK>(Bs, (wn * FN + j) * 32, kk, lane);
-      else fb[kk & 1][j] = frag_kr<BN>(Bs, (wn * FN + j) * 32, kk, lane);
+      if constexpr (FORM == 0) fb[set][j] = frag_kc<BK>(Bs, (wn * FN + j) * 32, kk, lane);
+      else fb[set][j] = frag_kr<BN>(Bs, (wn * FN + j) * 32, kk, lane);
     }
   };
   if (steps > 0) {
@@ -465,46 +462,46 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void a8_gemm16_kernel(A8Args a) {
 #pragma unroll
       for (int i = 0; i < FM; ++i)
 #pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = mfma16<T>(fb[kk & 1][j], fa[kk & 1][i], acc[i][j]);
+        for (int j = 0; j < FN; ++j) acc[i][j] = mfma16<T>(fb[kk % 2][j], fa[kk % 2][i], acc[i][j]);
       if constexpr (decltype(with_sums)::value) {
 #pragma unroll
-        for (int i = 0; i < FM; ++i) sum[i] = add8<T>(fa[kk & 1][i], sum[i]);
+        for (int i = 0; i < FM; ++i) sum[i] = add8<T>(fa[kk % 2][i], sum[i]);
       }
       __builtin_amdgcn_sched_barrier(0);
     };
     int buf = 0, s = 0;
     // steps with STAGES more behind them, without a branch
     for (; s + STAGES < steps; ++s) {
+      const int now = buf, before = now == 0 ? STAGES - 1 : now - 1;
 #pragma unroll
-      for (int kk = 0; kk + 1 < BK / 16; ++kk) {
+      for (int kk = 0; kk < KK; ++kk) {
+        if (kk == KK - 1) {             // the last fragments of this tile are under way: the border
+          buf = buf + 1 == STAGES ? 0 : buf + 1;
+          put_codes(before);            // what arrived during this step belongs to step s + STAGES - 1, in the buffer of the step before this one
+          wait_loads<LOADS * (STAGES - 2)>();
+          meet();
+        }
         read(buf, kk + 1);
+        if (kk == KK - 1) {
+          fetch(s_lo + s + STAGES);
+          issue(s_lo + s + STAGES, now);
+        }
         multiply(kk);
       }
-      const int now = buf, before = now == 0 ? STAGES - 1 : now - 1;
-      buf = buf + 1 == STAGES ? 0 : buf + 1;
-      put_codes(before);              // what arrived during this step belongs to step s + STAGES - 1, in the buffer of the step before this one
-      wait_loads<LOADS * (STAGES - 2)>();
-      meet();
-      read(buf, 0);
-      fetch(s_lo + s + STAGES);
-      issue(s_lo + s + STAGES, now);
-      multiply(BK / 16 - 1);
     }
     for (; s < steps; ++s) {
+      const int before = buf == 0 ? STAGES - 1 : buf - 1;
 #pragma unroll
-      for (int kk = 0; kk + 1 < BK / 16; ++kk) {
-        read(buf, kk + 1);
+      for (int kk = 0; kk < KK; ++kk) {
+        if (kk == KK - 1 && s + 1 < steps) {
+          buf = buf + 1 == STAGES ? 0 : buf + 1;
+          if (s + STAGES == steps) put_codes(before);
+          wait_loads<0>();              // (fewer loads behind the next step's than in the middle: wait for all)
+          meet();
+        }
+        if (kk < KK - 1 || s + 1 < steps) read(buf, kk + 1);
         multiply(kk);
       }
-      if (s + 1 < steps) {
-        const int before = buf == 0 ? STAGES - 1 : buf - 1;
-        buf = buf + 1 == STAGES ? 0 : buf + 1;
-        if (s + STAGES == steps) put_codes(before);
-        wait_loads<0>();              // (fewer loads behind the next step's than in the middle: wait for all)
-        meet();
-        read(buf, 0);
-      }
-      multiply(BK / 16 - 1);
     }
   };
   const bool sums = FORM == 2 && a.rowsum && t.n == 0 && wn == 0;
@@ -514,12 +511,42 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void a8_gemm16_kernel(A8Args a) {
   } else loop(std::false_type{});
   static_assert(FN == 2, "store_rows takes two blocks side by side");
   __syncthreads();                                         // the tiles have been read: their place is free
+  float *S = (float *)a8_lds;
+  if constexpr (WK == 2) {
+    // Each group stores half of the rows: it gives the other half's sums away, [wave of the group][FM / 2][FN][16][lane].
+    static_assert(FM % 2 == 0 && WK * WM * WN * (FM / 2) * (FN * 16 + 1) * 64 * 4 <= STAGES * STAGE * 2, "");
+    constexpr int EACH = (FM / 2) * (FN * 16 + 1) * 64;
+    float *give = S + wave * EACH + lane, *take = S + (wave ^ (WM * WN)) * EACH + lane;
+#pragma unroll
+    for (int i = 0; i < FM / 2; ++i) {
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) give[((i * FN + j) * 16 + r) * 64] = wk ? acc[i][j][r] : acc[FM / 2 + i][j][r];
+      give[((FM / 2) * FN * 16 + i) * 64] = wk ? sum[i] : sum[FM / 2 + i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < FM / 2; ++i) {
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float v = take[((i * FN + j) * 16 + r) * 64];
+          acc[i][j][r] = wk ? v + acc[FM / 2 + i][j][r] : acc[i][j][r] + v;      // (group 0 + group 1)
+        }
+      const float v = take[((FM / 2) * FN * 16 + i) * 64];
+      sum[i] = wk ? v + sum[FM / 2 + i] : sum[i] + v;
+    }
+    __syncthreads();
+  }
   float bias[8];
   load_bias<T>(a, n0 + wn * 64, lane, bias);
 #pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    store_rows<T>(a, t, acc[i][0], acc[i][1], (float *)a8_lds + wave * EPI_FLOATS, bias, m0 + (wm * FM + i) * 32, n0 + wn * 64, lane);
-    if (FORM == 2 && sums) store_sum<T>(a, t, sum[i], m0 + (wm * FM + i) * 32, lane);
+  for (int i = 0; i < FM / WK; ++i) {
+    const int m = m0 + (wm * FM + wk * (FM / WK) + i) * 32;
+    store_rows<T>(a, t, acc[i][0], acc[i][1], S + wave * EPI_FLOATS, bias, m, n0 + wn * 64, lane);
+    if (FORM == 2 && sums) store_sum<T>(a, t, sum[i], m, lane);
   }
 }
 
@@ -527,7 +554,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void a8_gemm16_kernel(A8Args a) {
 // 128 x 128 tile, 4 waves of 64 x 64, 32 of the contraction at a time; the next step's operands are in registers while this
 // one's planes are multiplied.
 template <int FORM>
-__global__ __launch_bounds__(256) void a8_gemm32_kernel(A8Args a) {
+__global__ __launch_bounds__(256, 3) void a8_gemm32_kernel(A8Args a) {
   constexpr int BM = 128, BN = 128, BK = 32, THREADS = 256, FM = 2, FN = 2, PB = FORM == 2 ? 1 : 3;
   extern __shared__ __attribute__((aligned(16))) uint16_t a8_lds[];
   uint16_t *As = a8_lds, *Bs = a8_lds + 3 * BM * BK;
@@ -579,8 +606,8 @@ __global__ __launch_bounds__(256) void a8_gemm32_kernel(A8Args a) {
       for (int q = 0; q < PB; ++q)
 #pragma unroll
         for (int j = 0; j < FN; ++j) {
-          if constexpr (FORM == 0) fb[q][j] = frag_kc<BK>(Bs + q * BN * BK, (wn * FN + j) * 32, kk, lane);
-          else fb[q][j] = frag_kr<BN>(Bs + q * BN * BK, (wn * FN + j) * 32, kk, lane);
+          if constexpr (FORM >= 1) fb[q][j] = frag_kr<BN>(Bs + q * BN * BK, (wn * FN + j) * 32, kk, lane);
+          else fb[q][j] = frag_kc<BK>(Bs + q * BN * BK, (wn * FN + j) * 32, kk, lane);
         }
       // smallest products first
 #pragma unroll
@@ -613,10 +640,14 @@ __global__ __launch_bounds__(256) void a8_gemm32_kernel(A8Args a) {
   }
 }
 
-// ---- partial sums, in split order ---------------------------------------------------------------------------------------
-// a thread has 4 neighbouring columns; the last workgroups take the row sums
-template <int T>
+// ---- partial sums, in a fixed order ---------------------------------------------------------------------------------------
+// A thread has 4 neighbouring columns and every SLICES-th part, 4 loads under way at a time; the slices are added in LDS.  Many parts of few
+// results are bound by the latency of that chain: 64 parts of 256 x 256 took 19 us one after the other.  The last workgroups take the
+// row sums.
+template <int T, int SLICES>
 __global__ __launch_bounds__(256) void a8_reduce_kernel(A8Args a, int col4, unsigned main_blocks) {
+  constexpr int THREADS = 256 / SLICES;
+  __shared__ float4 sh[SLICES > 1 ? 256 : 1];
   if (blockIdx.x >= main_blocks) {
     const long long m = (long long)(blockIdx.x - main_blocks) * 256 + threadIdx.x;
     if (m >= a.M) return;
@@ -626,25 +657,43 @@ __global__ __launch_bounds__(256) void a8_reduce_kernel(A8Args a, int col4, unsi
     act8_put<T>(a.rowsum, m, v);
     return;
   }
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const int tx = threadIdx.x % THREADS, slice = threadIdx.x / THREADS;
+  const long long i = (long long)blockIdx.x * THREADS + tx;
   const int m = (int)(i / col4), n = 4 * (int)(i % col4);     // col4: a multiple of 8 (a word of sign bits is 8 threads)
-  if (m >= a.M) return;
   float v[4] = {0.f, 0.f, 0.f, 0.f};
-  const float *p = a.part + (size_t)m * a.N + n;
-  for (int s = 0; s < a.splits; ++s, p += (size_t)a.M * a.N) {
-    if (a.N % 4 == 0 && n + 3 < a.N) {
-      const float4 w = *(const float4 *)p;
-      v[0] += w.x, v[1] += w.y, v[2] += w.z, v[3] += w.w;
-    } else {
+  if (m < a.M && n < a.N) {
+    const size_t step = (size_t)a.M * a.N * SLICES;
+    const float *p = a.part + ((size_t)slice * a.M + m) * a.N + n;
+    const bool whole = a.N % 4 == 0;
+    int s = slice;
+    if (whole) {
+      for (; s + 3 * SLICES < a.splits; s += 4 * SLICES, p += 4 * step) {
+        const float4 w0 = *(const float4 *)p, w1 = *(const float4 *)(p + step), w2 = *(const float4 *)(p + 2 * step), w3 = *(const float4 *)(p + 3 * step);
+        v[0] += (w0.x + w1.x) + (w2.x + w3.x), v[1] += (w0.y + w1.y) + (w2.y + w3.y);
+        v[2] += (w0.z + w1.z) + (w2.z + w3.z), v[3] += (w0.w + w1.w) + (w2.w + w3.w);
+      }
+    }
+    for (; s < a.splits; s += SLICES, p += step) {
 #pragma unroll
       for (int k = 0; k < 4; ++k)
         if (n + k < a.N) v[k] += p[k];
     }
   }
-  finish4<T>(a, m, n, v);
+  if constexpr (SLICES > 1) {
+    sh[threadIdx.x] = make_float4(v[0], v[1], v[2], v[3]);
+    __syncthreads();
+    if (slice) return;
+#pragma unroll
+    for (int k = 1; k < SLICES; ++k) {
+      const float4 w = sh[k * THREADS + tx];
+      v[0] += w.x, v[1] += w.y, v[2] += w.z, v[3] += w.w;
+    }
+  }
+  if (m >= a.M) return;
   uint32_t word = 0;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
+    if (a.bias && n + k < a.N) v[k] += act8_get<T>(a.bias, n + k);
     if (v[k] > 0.f) word |= 1u << ((n & 31) + k);
     if (a.relu) v[k] = v[k] < 0.f ? 0.f : v[k];
   }
@@ -676,30 +725,22 @@ __global__ __launch_bounds__(256) void a8_mask_kernel(const void *__restrict__ x
   }
 }
 
-#ifndef A8_BIG_TILES
-#define A8_BIG_TILES 200   // large tiles from so many of them on
-#endif
-#ifndef A8_SBK
-#define A8_SBK 64
-#endif
-#ifndef A8_SST
-#define A8_SST 2
-#endif
-#ifndef A8_BIG2
-#define A8_BIG2 2, 2, 4, 2, 32, 3
-#endif
-#ifndef A8_BIG0
-#define A8_BIG0 2, 4, 4, 2, 64, 2
-#endif
+// Large tiles where there are this many of them: 256 x 256 for forms 0 and 1 (rows of 128 bytes a step: 32 of the contraction read half of each
+// 128-byte line at a time, 776 against 863 TFLOP/s at 16 384 x 4 096 x 4 096), 256 x 128 with two workgroups to a compute unit for form 2
+// (1 047 TFLOP/s there; the 256 x 256 tile spills: 535).
+constexpr int A8_BIG_TILES = 200;
 
-template <int WM_, int WN_, int FM_, int FN_, int BK_, int STAGES_>
+template <int WM_, int WN_, int FM_, int FN_, int BK_, int STAGES_, int WK_>
 struct Shape {
-  static constexpr int WM = WM_, WN = WN_, FM = FM_, FN = FN_, BK = BK_, STAGES = STAGES_, BM = WM * FM * 32, BN = WN * FN * 32,
-                       THREADS = 64 * WM * WN, LDS = STAGES * (BM + BN) * BK * 2;
+  static constexpr int WM = WM_, WN = WN_, FM = FM_, FN = FN_, BK = BK_, STAGES = STAGES_, WK = WK_, BM = WM * FM * 32, BN = WN * FN * 32,
+                       THREADS = 64 * WM * WN * WK, TILES = STAGES * (BM + BN) * BK * 2, ROWS = WK * WM * WN * EPI_FLOATS * 4,
+                       LDS = TILES > ROWS ? TILES : ROWS;
 };
-typedef Shape<2, 2, 2, 2, A8_SBK, A8_SST> Small;
-typedef Shape<A8_BIG0> BigForward;      // forms 0 and 1
-typedef Shape<A8_BIG2> BigWeight;       // form 2
+// Fewer results: 128 x 128, 8 waves in two groups that share the contraction (4 096 x 1 024 results of a product over 4 096, us of forms 0 / 1 / 2: 4
+// waves and two stages 50 / 66 / 74, 8 waves of 32 x 64 and four stages 41 / 60 / 69, this 41 / 55 / 63).
+typedef Shape<2, 2, 2, 2, 64, 4, 2> Small;
+typedef Shape<2, 4, 4, 2, 64, 2, 1> BigForward;
+typedef Shape<2, 2, 4, 2, 32, 3, 1> BigWeight;
 
 constexpr long long A8_MAX_PITCH = (1ll << 31) / 512 - 8;
 
@@ -720,7 +761,8 @@ Plan a8_plan(int form, int dtype, int M, int N, int K) {
   p.tiles_m = dm_ceil_div(M, p.bm), p.tiles_n = dm_ceil_div(N, p.bn);
   const long long tiles = (long long)p.tiles_m * p.tiles_n;
   const int steps = dm_ceil_div(K, p.bk);
-  long long want = p.big || tiles >= 256 ? 1 : (512 + tiles - 1) / tiles;
+  const int fill = dtype == ACT8_F32 ? 512 : 256;                       // workgroups that are resident at once, about
+  long long want = p.big || tiles >= 256 ? 1 : (fill + tiles - 1) / tiles;
   const long long most = (long long)steps * p.bk / 256;                 // a split has 256 of the contraction at least
   if (want > most) want = most;
   if (want > 64) want = 64;
@@ -732,7 +774,7 @@ Plan a8_plan(int form, int dtype, int M, int N, int K) {
 
 template <int T, int FORM, typename S>
 int launch16(const A8Args &a, unsigned grid, hipStream_t st) {
-  auto k = a8_gemm16_kernel<T, FORM, S::WM, S::WN, S::FM, S::FN, S::BK, S::STAGES>;
+  auto k = a8_gemm16_kernel<T, FORM, S::WM, S::WN, S::FM, S::FN, S::BK, S::STAGES, S::WK>;
   if (S::LDS > 65536) DM_HIP(hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS));
   k<<<grid, S::THREADS, S::LDS, st>>>(a);
   DM_CHECK_LAUNCH();
@@ -756,9 +798,10 @@ int launch32(const A8Args &a, unsigned grid, hipStream_t st) {
 
 template <int T>
 int reduce(const A8Args &a, hipStream_t st) {
-  const int col4 = dm_ceil_div(a.N, 32) * 8;
-  const long long main_blocks = ((long long)a.M * col4 + 255) / 256, more = a.rowsum ? (a.M + 255) / 256 : 0;
-  a8_reduce_kernel<T><<<(unsigned)(main_blocks + more), 256, 0, st>>>(a, col4, (unsigned)main_blocks);
+  const int col4 = dm_ceil_div(a.N, 32) * 8, threads = a.splits >= 8 ? 64 : 256;
+  const long long main_blocks = ((long long)a.M * col4 + threads - 1) / threads, more = a.rowsum ? (a.M + 255) / 256 : 0;
+  if (threads == 64) a8_reduce_kernel<T, 4><<<(unsigned)(main_blocks + more), 256, 0, st>>>(a, col4, (unsigned)main_blocks);
+  else a8_reduce_kernel<T, 1><<<(unsigned)(main_blocks + more), 256, 0, st>>>(a, col4, (unsigned)main_blocks);
   DM_CHECK_LAUNCH();
   return DM_OK;
 }
@@ -797,7 +840,7 @@ extern "C" int dm_act8_gemm(int form, int dtype, const void *A, long long lda, c
     a.part = (float *)workspace;
   }
   const long long total = (long long)p.tiles_m * p.tiles_n * p.splits;
-  if (total > 0x3fffffff || (long long)M * (dm_ceil_div(N, 32) * 8) / 256 > 0x7ffffff0) return DM_ERR_INVALID_ARG;
+  if (total > 0x3fffffff || (long long)M * (dm_ceil_div(N, 32) * 8) / 64 > 0x7ffffff0) return DM_ERR_INVALID_ARG;
   a.per_xcd = (int)((total + 7) / 8);
   const unsigned grid = (unsigned)a.per_xcd * 8;
   int rc;
