@@ -203,8 +203,8 @@ SIGNATURES = {
     'dm_multi_add_f32': (ci, [vp, ci, ctypes.c_longlong, ci, vp]),
     'dm_act8_pack': (ci, [vp, ci, ctypes.c_longlong, ci, ctypes.c_longlong, vp, vp, vp]),
     'dm_act8_unpack': (ci, [vp, vp, ctypes.c_longlong, ci, vp, ci, vp]),
-    'dm_act8_gemm_workspace_bytes': (sz, [ci, ci, ci, ci, ci]),
-    'dm_act8_gemm': (ci, [ci, ci, vp, ctypes.c_longlong, vp, ctypes.c_longlong, vp, vp, ci, ci, ci, ci, vp, vp, vp, vp, sz, vp]),
+    'dm_act8_gemm_workspace_bytes': (sz, [ci, ci, vp, ctypes.c_longlong, vp, ctypes.c_longlong, ci, ci, ci, ci]),
+    'dm_act8_gemm': (ci, [ci, ci, vp, ctypes.c_longlong, vp, ctypes.c_longlong, ci, vp, vp, ci, ci, ci, ci, vp, vp, vp, vp, sz, vp]),
     'dm_block_norm_max_width': (ci, []),
     'dm_block_norm_forward': (ci, [ctypes.POINTER(BlockNorm), vp, ctypes.c_longlong, vp, ctypes.c_longlong, vp, vp, vp]),
     'dm_block_norm_workspace_bytes': (sz, [ctypes.c_longlong, ci, ctypes.c_longlong]),

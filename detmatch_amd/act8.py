@@ -133,46 +133,59 @@ def unpack(kept, dtype=None):
 _MAX = (1 << 31) - 1024                      # rows and channels are 32-bit numbers in the kernels
 
 
-def _operand(r, dtype_code):
-    """(tensor, pitch) of rows that dm_act8_gemm reads: r itself, or for 16-bit rows that 16-byte reads do not fit, a copy
-    with a pitch of 8 elements and zeros behind the width."""
-    pitch = row_stride(r)
-    if dtype_code == 0 or (r.shape[1] % 8 == 0 and pitch % 8 == 0 and r.data_ptr() % 16 == 0):
-        return r, pitch
-    return _masked(r, None, dtype_code)
+_COPY_FROM = 1 << 33                         # multiply-adds; see _operands
 
 
-def _masked(r, bits, dtype_code):
-    rows, width = r.shape
+def _operand(r):
+    """(tensor to keep alive, address, pitch) of rows as they lie."""
+    r = rows_view(r)
+    return r, r.data_ptr(), row_stride(r)
+
+
+def _direct(o, width):
+    return width % 8 == 0 and o[2] % 8 == 0 and o[1] % 16 == 0
+
+
+def _masked(o, rows, width, bits, code):
+    """A copy of an operand with a pitch of 8 elements and zeros behind its width, and 0 where a sign bit is not set."""
+    r = o[0]
     pitch = (width + 7) // 8 * 8
     out = torch.empty((rows, pitch), dtype=r.dtype, device=r.device)
-    _lib.check(_lib.lib().dm_act8_mask_rows(_lib.ptr(r), dtype_code, rows, width, row_stride(r), _lib.ptr(bits), _lib.ptr(out),
-                                            pitch, _lib.stream()), 'dm_act8_mask_rows')
-    return out, pitch
+    at = out.data_ptr()
+    _lib.check(_lib.lib().dm_act8_mask_rows(o[1], code, rows, width, o[2], bits, at, pitch,
+                                            _lib.raw_stream()), 'dm_act8_mask_rows')
+    return out, at, pitch
 
 
-def _gemm(form, code, a, b, exps, bias, relu, m, n, k, out, bits=None, rowsum=None):
-    """a, b: (tensor, pitch)"""
+def _gemm(form, code, a, b, exps, bias, relu, m, n, k, out, bits=None, rowsum=None, masked=False):
+    """One product; a, b: (what to keep alive, address, pitch); exps, bias, bits, rowsum: addresses or None; masked: a is _masked's."""
+    padded = 1 if masked else 0
+    if code and m * n * k >= _COPY_FROM:
+        # Rows at any address go through registers, and through small tiles: for large products a copy at 16-byte pitch and the direct
+        # path are faster.
+        wide = m if form == 2 else k
+        if not masked and not _direct(a, wide):
+            a, padded = _masked(a, k if form == 2 else m, wide, None, code), 1
+        wide = k if form == 0 else n
+        if form != 2 and not _direct(b, wide):
+            b, padded = _masked(b, n if form == 0 else k, wide, None, code), padded | 2
     L = _lib.lib()
-    need = int(L.dm_act8_gemm_workspace_bytes(form, code, m, n, k))
+    need = L.dm_act8_gemm_workspace_bytes(form, code, a[1], a[2], b[1], b[2], padded, m, n, k)
     # (a buffer of its own for every call: two streams, or two captured graphs, never share one)
     ws = torch.empty(need, dtype=torch.uint8, device=out.device) if need else None
-    _lib.check(L.dm_act8_gemm(form, code, _lib.ptr(a[0]), a[1], _lib.ptr(b[0]), b[1], _lib.ptr(exps), _lib.ptr(bias), int(relu), m, n,
-                              k, _lib.ptr(out), _lib.ptr(bits), _lib.ptr(rowsum), _lib.ptr(ws), need, _lib.stream()), 'dm_act8_gemm')
+    e = L.dm_act8_gemm(form, code, a[1], a[2], b[1], b[2], padded, exps, bias, relu, m, n, k, out.data_ptr(), bits, rowsum,
+                       ws.data_ptr() if need else None, need, _lib.raw_stream())
+    if e:
+        _lib.check(e, 'dm_act8_gemm')
     return out
 
 
-def _linear_forward(x, w, b, relu, keep, bits):
-    """y, and of x (rows, in) what `keep` asks for (an Act8 or None); bits: write the sign bits of y (or None)."""
-    code = DTYPES[x.dtype]
-    m, k = x.shape
-    n = w.shape[0]
-    y = torch.empty((m, n), dtype=x.dtype, device=x.device)
-    kept = pack(x) if keep else None
-    if m:
-        _gemm(0, code, _operand(rows_view(x), code), _operand(rows_view(w), code), None, None if b is None else b.contiguous(), relu, m, n, k,
-              y, bits)
-    return y, kept
+def _kept_layout(m, n, k, codes, bits):
+    """Offsets of codes, exponents and sign bits in the one buffer that a layer keeps, and its size."""
+    groups = (k + GROUP - 1) // GROUP
+    at_exps = m * groups * GROUP if codes else 0
+    at_bits = (at_exps + (m * groups if codes else 0) + 3) // 4 * 4
+    return groups, at_exps, at_bits, at_bits + (m * ((n + 31) // 32) * 4 if bits else 0)
 
 
 class _Linear8(Function):
@@ -180,19 +193,31 @@ class _Linear8(Function):
     @staticmethod
     def forward(ctx, x, w, b, relu):
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        m, n = x.shape[0], w.shape[0]
-        with _on(x.device):
-            bits = torch.empty((m, (n + 31) // 32), dtype=torch.int32, device=x.device) if relu else None
-            y, kept = _linear_forward(x, w, b, relu, need_w, bits)
-        ctx.save_for_backward(w if need_x else None, kept.codes if kept else None, kept.exps if kept else None, bits)
-        ctx.sizes = (m, n, x.shape[1])
+        m, k = x.shape
+        n = w.shape[0]
+        dev, code = x.device, DTYPES[x.dtype]
+        groups, at_exps, at_bits, size = _kept_layout(m, n, k, need_w, relu)
+        with _on(dev):
+            kept = torch.empty(size, dtype=torch.uint8, device=dev)
+            y = torch.empty((m, n), dtype=x.dtype, device=dev)
+            if m:
+                base, xo = kept.data_ptr(), _operand(x)
+                if need_w:
+                    e = _lib.lib().dm_act8_pack(xo[1], code, m, k, xo[2], base, base + at_exps, _lib.raw_stream())
+                    if e:
+                        _lib.check(e, 'dm_act8_pack')
+                bias = None if b is None else b.contiguous()
+                _gemm(0, code, xo, _operand(w), None, None if b is None else bias.data_ptr(), relu, m, n, k, y,
+                      base + at_bits if relu else None)
+        ctx.save_for_backward(w if need_x else None, kept)
+        ctx.rest = (m, n, k, relu)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gy):
-        w, codes, exps, bits = ctx.saved_tensors
-        m, n, k = ctx.sizes
+        w, kept = ctx.saved_tensors
+        m, n, k, relu = ctx.rest
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         code, dtype, dev = DTYPES[gy.dtype], gy.dtype, gy.device
         gx = gw = gb = None
@@ -200,19 +225,21 @@ class _Linear8(Function):
             if m == 0:
                 return (gy.new_zeros((0, k)) if need_x else None, gy.new_zeros((n, k)) if need_w else None,
                         gy.new_zeros(n) if need_b else None, None)
-            g = rows_view(gy)
-            g = _operand(g, code) if bits is None else _masked(g, bits, code)
+            groups, at_exps, at_bits, _ = _kept_layout(m, n, k, need_w, relu)
+            base, g = kept.data_ptr(), _operand(gy)
+            if relu:
+                g = _masked(g, m, n, base + at_bits, code)
             if need_x:
-                gx = _gemm(1, code, g, _operand(rows_view(w), code), None, None, False, m, k, n, torch.empty((m, k), dtype=dtype, device=dev))
-            if need_w or need_b:
-                gb = torch.empty(n, dtype=dtype, device=dev) if need_b else None
-                if need_w:
-                    gw = _gemm(2, code, g, (codes, codes.shape[1]), exps, None, False, n, k, m,
-                               torch.empty((n, k), dtype=dtype, device=dev), rowsum=gb)
-                else:                         # a bias alone: its sums ride on a product with one group of zeros
-                    zero = torch.zeros((2, m, GROUP), dtype=torch.uint8, device=dev)
-                    _gemm(2, code, g, (zero[0], GROUP), zero[1], None, False, n, GROUP, m,
-                          torch.empty((n, GROUP), dtype=dtype, device=dev), rowsum=gb)
+                gx = _gemm(1, code, g, _operand(w), None, None, 0, m, k, n, torch.empty((m, k), dtype=dtype, device=dev), masked=relu)
+            if need_b:
+                gb = torch.empty(n, dtype=dtype, device=dev)
+            if need_w:
+                gw = _gemm(2, code, g, (kept, base, groups * GROUP), base + at_exps, None, 0, n, k, m,
+                           torch.empty((n, k), dtype=dtype, device=dev), rowsum=gb.data_ptr() if need_b else None, masked=relu)
+            elif need_b:                      # a bias alone: its sums ride on a product with one group of zeros
+                zero = torch.zeros((2, m, GROUP), dtype=torch.uint8, device=dev)
+                _gemm(2, code, g, (zero, zero.data_ptr(), GROUP), zero.data_ptr() + m * GROUP, None, 0, n, GROUP, m,
+                      torch.empty((n, GROUP), dtype=dtype, device=dev), rowsum=gb.data_ptr(), masked=relu)
         return gx, gw, gb, None
 
 
@@ -239,6 +266,11 @@ def linear(x, w, b=None, relu=False):
     if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or (b is not None and b.requires_grad)):
         y = _Linear8.apply(x2, w, b, bool(relu))
     else:
+        m, k = x2.shape
+        n = w.shape[0]
         with _on(x.device):
-            y, _ = _linear_forward(x2, w, b, bool(relu), False, None)
+            y = torch.empty((m, n), dtype=x.dtype, device=x.device)
+            if m:
+                bias = None if b is None else b.contiguous()
+                _gemm(0, DTYPES[x.dtype], _operand(x2), _operand(w), None, None if b is None else bias.data_ptr(), bool(relu), m, n, k, y)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], w.shape[0])

@@ -165,6 +165,36 @@ struct Stager {
   }
 };
 
+// The same through registers, for rows at any address: 8 elements a thread, any alignment, nothing read behind a row's end.
+template <int T, bool ALONG_K, int SIDE, int BK, int THREADS>
+struct RowRegs {
+  static constexpr int H = SIDE * BK / 8 / THREADS;
+  Act8Raw<T> r[H];
+
+  __device__ __forceinline__ void fetch(const uint16_t *P, long long ld, int side0, int side, int k0, int k_hi, int tid) {
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      const int i = tid + THREADS * h;
+      if (!ALONG_K) {
+        const int row = side0 + i / (BK / 8), k = k0 + 8 * (i % (BK / 8));
+        r[h] = act8_load_raw<T>(P, (size_t)((long long)row * ld + k), row < side ? k_hi - k : 0);
+      } else {
+        const int k = k0 + i / (SIDE / 8), c = side0 + 8 * (i % (SIDE / 8));
+        r[h] = act8_load_raw<T>(P, (size_t)((long long)k * ld + c), k < k_hi ? side - c : 0);
+      }
+    }
+  }
+
+  __device__ __forceinline__ void put(uint16_t *S, int tid) const {
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      const int i = tid + THREADS * h, row = ALONG_K ? i / (SIDE / 8) : i / (BK / 8);
+      const int c = ALONG_K ? (i % (SIDE / 8)) ^ kr_swizzle(row) : (i % (BK / 8)) ^ kc_swizzle<BK>(row);
+      *(act8_u32x4 *)(S + row * (ALONG_K ? SIDE : BK) + c * 8) = r[h].w[0];
+    }
+  }
+};
+
 // 8-bit operand: 16 codes of a row at a time through registers
 template <int COLS, int BK, int THREADS>
 struct CodeRegs {
@@ -382,8 +412,8 @@ __device__ __forceinline__ void store_sum(const A8Args &a, const Tile &t, float 
   else act8_put<T>(a.rowsum, m, v);
 }
 
-// WK groups of WM x WN waves share a tile: each multiplies its part of every step's contraction, and they add up at the end.
-template <int T, int FORM, int WM, int WN, int FM, int FN, int BK, int STAGES, int WK>
+// REGS: operands at any address, through registers.  WK groups of WM x WN waves share a tile: each multiplies its part of every step's contraction, and they add up at the end.
+template <int T, int FORM, int WM, int WN, int FM, int FN, int BK, int STAGES, int WK, bool REGS>
 __global__ __launch_bounds__(64 * WM * WN * WK, 2) void a8_gemm16_kernel(A8Args a) {
   constexpr int BM = WM * FM * 32, BN = WN * FN * 32, THREADS = 64 * WM * WN * WK, STAGE = (BM + BN) * BK;
   extern __shared__ __attribute__((aligned(16))) uint16_t a8_lds[];      // [STAGES][A tile, B tile]
@@ -407,19 +437,34 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void a8_gemm16_kernel(A8Args 
   typedef Stager<FORM == 1, BN, BK, THREADS> SB;
   SA sa;
   SB sb;
+  RowRegs<T, FORM == 2, BM, BK, THREADS> ra;
+  RowRegs<T, FORM == 1, BN, BK, THREADS> rb;
   CodeRegs<BN, BK, THREADS> codes;
-  constexpr int LOADS = SA::H + (FORM == 2 ? 0 : SB::H);
-  sa.start((const uint16_t *)a.A, a.lda, m0, a.M, s_lo * BK, tid);
-  if constexpr (FORM != 2) sb.start((const uint16_t *)a.B, a.ldb, n0, a.N, s_lo * BK, tid);
+  constexpr int LOADS = REGS ? 0 : SA::H + (FORM == 2 ? 0 : SB::H);
+  if constexpr (!REGS) {
+    sa.start((const uint16_t *)a.A, a.lda, m0, a.M, s_lo * BK, tid);
+    if constexpr (FORM != 2) sb.start((const uint16_t *)a.B, a.ldb, n0, a.N, s_lo * BK, tid);
+  }
 
+  // what goes through registers: fetched one step before put stores it
   auto fetch = [&](int s) {
+    if constexpr (REGS) {
+      ra.fetch((const uint16_t *)a.A, a.lda, m0, a.M, s * BK, a.K, tid);
+      if constexpr (FORM != 2) rb.fetch((const uint16_t *)a.B, a.ldb, n0, a.N, s * BK, a.K, tid);
+    }
     if constexpr (FORM == 2) fetch_codes<BN, BK, THREADS>(codes, (const uint8_t *)a.B, a.exps, a.ldb, n0, s * BK, a.K, tid);
   };
   auto issue = [&](int s, int buf) {
-    sa.issue(a8_lds + buf * STAGE, wave, a.K - s * BK);
-    if constexpr (FORM != 2) sb.issue(a8_lds + buf * STAGE + BM * BK, wave, a.K - s * BK);
+    if constexpr (!REGS) {
+      sa.issue(a8_lds + buf * STAGE, wave, a.K - s * BK);
+      if constexpr (FORM != 2) sb.issue(a8_lds + buf * STAGE + BM * BK, wave, a.K - s * BK);
+    }
   };
-  auto put_codes = [&](int buf) {
+  auto put = [&](int buf) {
+    if constexpr (REGS) {
+      ra.put(a8_lds + buf * STAGE, tid);
+      if constexpr (FORM != 2) rb.put(a8_lds + buf * STAGE + BM * BK, tid);
+    }
     if constexpr (FORM == 2) store_codes<T, BN, BK, THREADS>(codes, a8_lds + buf * STAGE + BM * BK, tid);
   };
 
@@ -429,7 +474,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void a8_gemm16_kernel(A8Args 
     if (i < steps) {
       fetch(s_lo + i);
       issue(s_lo + i, i);
-      if (i < STAGES - 1) put_codes(i);                    // (the last ones wait in registers)
+      if (i < STAGES - 1) put(i);                    // (the last ones wait in registers)
     }
   }
   constexpr int KK = BK / 16 / WK;                         // groups of 16 that a wave multiplies of a step
@@ -477,7 +522,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void a8_gemm16_kernel(A8Args 
       for (int kk = 0; kk < KK; ++kk) {
         if (kk == KK - 1) {             // the last fragments of this tile are under way: the border
           buf = buf + 1 == STAGES ? 0 : buf + 1;
-          put_codes(before);            // what arrived during this step belongs to step s + STAGES - 1, in the buffer of the step before this one
+          put(before);            // what arrived during this step belongs to step s + STAGES - 1, in the buffer of the step before this one
           wait_loads<LOADS * (STAGES - 2)>();
           meet();
         }
@@ -495,7 +540,7 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void a8_gemm16_kernel(A8Args 
       for (int kk = 0; kk < KK; ++kk) {
         if (kk == KK - 1 && s + 1 < steps) {
           buf = buf + 1 == STAGES ? 0 : buf + 1;
-          if (s + STAGES == steps) put_codes(before);
+          if (s + STAGES == steps) put(before);
           wait_loads<0>();              // (fewer loads behind the next step's than in the middle: wait for all)
           meet();
         }
@@ -748,12 +793,12 @@ struct Plan {
   int big, bm, bn, bk, tiles_m, tiles_n, splits, steps_per_split;
 };
 
-Plan a8_plan(int form, int dtype, int M, int N, int K) {
+Plan a8_plan(int form, int dtype, bool regs, int M, int N, int K) {
   Plan p;
   p.bm = p.bn = 128;
   p.bk = dtype == ACT8_F32 ? 32 : Small::BK;
   p.big = 0;
-  if (dtype != ACT8_F32) {
+  if (dtype != ACT8_F32 && !regs) {
     const int bm = form == 2 ? BigWeight::BM : BigForward::BM, bn = form == 2 ? BigWeight::BN : BigForward::BN;
     if ((long long)dm_ceil_div(M, bm) * dm_ceil_div(N, bn) >= A8_BIG_TILES)
       p.big = 1, p.bm = bm, p.bn = bn, p.bk = form == 2 ? BigWeight::BK : BigForward::BK;
@@ -763,7 +808,9 @@ Plan a8_plan(int form, int dtype, int M, int N, int K) {
   const int steps = dm_ceil_div(K, p.bk);
   const int fill = dtype == ACT8_F32 ? 512 : 256;                       // workgroups that are resident at once, about
   long long want = p.big || tiles >= 256 ? 1 : (fill + tiles - 1) / tiles;
-  const long long most = (long long)steps * p.bk / 256;                 // a split has 256 of the contraction at least
+  // A split has 256 of the contraction at least, and a short contraction is not worth the second kernel (1 024^3 bf16: 13.5 us, split 20; 256 x 2 000
+  // x 256 bf16: 20, split 13; through registers, a step's loads are not hidden as well: 777 x 1 001 x 515 fp16 25, split 18, fp32 78 and 31).
+  const long long most = K < (dtype == ACT8_F32 || regs ? 512 : 1536) ? 1 : (long long)steps * p.bk / 256;
   if (want > most) want = most;
   if (want > 64) want = 64;
   if (want < 1) want = 1;
@@ -772,9 +819,9 @@ Plan a8_plan(int form, int dtype, int M, int N, int K) {
   return p;
 }
 
-template <int T, int FORM, typename S>
+template <int T, int FORM, typename S, bool REGS = false>
 int launch16(const A8Args &a, unsigned grid, hipStream_t st) {
-  auto k = a8_gemm16_kernel<T, FORM, S::WM, S::WN, S::FM, S::FN, S::BK, S::STAGES, S::WK>;
+  auto k = a8_gemm16_kernel<T, FORM, S::WM, S::WN, S::FM, S::FN, S::BK, S::STAGES, S::WK, REGS>;
   if (S::LDS > 65536) DM_HIP(hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS));
   k<<<grid, S::THREADS, S::LDS, st>>>(a);
   DM_CHECK_LAUNCH();
@@ -782,7 +829,9 @@ int launch16(const A8Args &a, unsigned grid, hipStream_t st) {
 }
 
 template <int T>
-int launch16(int form, const A8Args &a, const Plan &p, unsigned grid, hipStream_t st) {
+int launch16(int form, bool regs, const A8Args &a, const Plan &p, unsigned grid, hipStream_t st) {
+  if (regs)
+    return form == 0 ? launch16<T, 0, Small, true>(a, grid, st) : form == 1 ? launch16<T, 1, Small, true>(a, grid, st) : launch16<T, 2, Small, true>(a, grid, st);
   if (form == 0) return p.big ? launch16<T, 0, BigForward>(a, grid, st) : launch16<T, 0, Small>(a, grid, st);
   if (form == 1) return p.big ? launch16<T, 1, BigForward>(a, grid, st) : launch16<T, 1, Small>(a, grid, st);
   return p.big ? launch16<T, 2, BigWeight>(a, grid, st) : launch16<T, 2, Small>(a, grid, st);
@@ -808,13 +857,25 @@ int reduce(const A8Args &a, hipStream_t st) {
 
 }  // namespace
 
-extern "C" size_t dm_act8_gemm_workspace_bytes(int form, int dtype, int M, int N, int K) {
+// rows that 16-byte loads straight into LDS fit: every address a multiple of 16, a tile's 256 rows less than 2^31 bytes; `whole`: no row ends inside
+// of a 16-byte piece, or (padded) what is behind its end may be read
+static bool a8_direct(const void *p, long long ld, int whole, int padded) {
+  return ld % 8 == 0 && ld <= A8_MAX_PITCH && ((uintptr_t)p & 15) == 0 && (padded || whole % 8 == 0);
+}
+
+static bool a8_regs(int form, int dtype, const void *A, long long lda, const void *B, long long ldb, int padded, int M, int N, int K) {
+  if (dtype == ACT8_F32) return false;
+  return !a8_direct(A, lda, form == 2 ? M : K, padded & 1) || (form != 2 && !a8_direct(B, ldb, form == 0 ? K : N, padded & 2));
+}
+
+extern "C" size_t dm_act8_gemm_workspace_bytes(int form, int dtype, const void *A, long long lda, const void *B, long long ldb, int padded, int M,
+                                               int N, int K) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  const Plan p = a8_plan(form, dtype, M, N, K);
+  const Plan p = a8_plan(form, dtype, a8_regs(form, dtype, A, lda, B, ldb, padded, M, N, K), M, N, K);
   return p.splits > 1 ? dm_align(((size_t)p.splits * M * N + (form == 2 ? (size_t)p.splits * M : 0)) * sizeof(float)) : 0;
 }
 
-extern "C" int dm_act8_gemm(int form, int dtype, const void *A, long long lda, const void *B, long long ldb, const uint8_t *exps,
+extern "C" int dm_act8_gemm(int form, int dtype, const void *A, long long lda, const void *B, long long ldb, int padded, const uint8_t *exps,
                             const void *bias, int relu, int M, int N, int K, void *C, uint32_t *sign_bits, void *rowsum,
                             void *workspace, size_t workspace_bytes, dm_stream_t stream) {
   hipStream_t st = (hipStream_t)stream;
@@ -823,20 +884,15 @@ extern "C" int dm_act8_gemm(int form, int dtype, const void *A, long long lda, c
   if ((form == 2) != (exps != nullptr) || (form != 2 && rowsum) || (form == 2 && (bias || relu || sign_bits))) return DM_ERR_INVALID_ARG;
   if (lda < (form == 2 ? M : K) || ldb < (form == 0 ? K : N)) return DM_ERR_INVALID_ARG;
   if (form == 2 && (ldb % 32 || ((uintptr_t)B & 15))) return DM_ERR_INVALID_ARG;
+  const bool regs = a8_regs(form, dtype, A, lda, B, ldb, padded, M, N, K);
+  const Plan p = a8_plan(form, dtype, regs, M, N, K);
   A8Args a = {};
-  if (dtype != ACT8_F32) {
-    // 16-byte pieces: no piece crosses a row's end (the pitch has room for the last one), every address is a multiple of 16, and a tile's
-    // 256 rows are less than 2^31 bytes
-    if (lda > A8_MAX_PITCH || (form != 2 && ldb > A8_MAX_PITCH)) return DM_ERR_UNSUPPORTED;
-    if (lda % 8 || ((uintptr_t)A & 15) || (form != 2 && (ldb % 8 || ((uintptr_t)B & 15)))) return DM_ERR_UNSUPPORTED;
-  }
-  const Plan p = a8_plan(form, dtype, M, N, K);
   a.A = A, a.B = B, a.bias = bias, a.exps = exps, a.C = C, a.bits = sign_bits, a.rowsum = rowsum;
   a.M = M, a.N = N, a.K = K, a.lda = lda, a.ldb = ldb, a.relu = relu;
   a.splits = p.splits, a.steps_per_split = p.steps_per_split, a.tiles_m = p.tiles_m, a.tiles_n = p.tiles_n;
   a.vec_c = N % 4 == 0 && ((uintptr_t)C & 15) == 0;
   if (p.splits > 1) {
-    if (!workspace || workspace_bytes < dm_act8_gemm_workspace_bytes(form, dtype, M, N, K)) return DM_ERR_WORKSPACE;
+    if (!workspace || workspace_bytes < dm_act8_gemm_workspace_bytes(form, dtype, A, lda, B, ldb, padded, M, N, K)) return DM_ERR_WORKSPACE;
     a.part = (float *)workspace;
   }
   const long long total = (long long)p.tiles_m * p.tiles_n * p.splits;
@@ -845,7 +901,7 @@ extern "C" int dm_act8_gemm(int form, int dtype, const void *A, long long lda, c
   const unsigned grid = (unsigned)a.per_xcd * 8;
   int rc;
   if (dtype == ACT8_F32) rc = form == 0 ? launch32<0>(a, grid, st) : form == 1 ? launch32<1>(a, grid, st) : launch32<2>(a, grid, st);
-  else rc = dtype == ACT8_BF16 ? launch16<ACT8_BF16>(form, a, p, grid, st) : launch16<ACT8_F16>(form, a, p, grid, st);
+  else rc = dtype == ACT8_BF16 ? launch16<ACT8_BF16>(form, regs, a, p, grid, st) : launch16<ACT8_F16>(form, regs, a, p, grid, st);
   if (rc != DM_OK || p.splits == 1) return rc;
   return dtype == ACT8_F32 ? reduce<ACT8_F32>(a, st) : dtype == ACT8_BF16 ? reduce<ACT8_BF16>(a, st) : reduce<ACT8_F16>(a, st);
 }

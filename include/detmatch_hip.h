@@ -1112,14 +1112,16 @@ int dm_act8_unpack(const uint8_t *codes, const uint8_t *exps, long long rows, in
  *   form 1  C[M][N] = A[M][K] . B[K][N]
  *   form 2  C[M][N] = A[K][M]^T . deq(B)[K][N]                 B codes, row pitch ldb = 32 * groups, exps (K, groups) as
  *                                                              dm_act8_pack writes them; rowsum (M) or NULL: sums of A's columns
- * Rows of A and B have pitches lda, ldb; C is dense.  16-bit operands: addresses multiples of 16 bytes, pitches of 8 elements
- * (else DM_ERR_UNSUPPORTED), rows readable up to the next multiple of 8 elements, and 0 there where they run along the contraction
- * (dm_act8_mask_rows without bits makes such a copy).  Few output tiles: the contraction is split and the parts (workspace) are
- * added in order; results depend on shapes and values alone.
+ * Rows of A and B have pitches lda, ldb; C is dense.  16-bit operands at any address; those whose addresses are multiples of 16 bytes, whose pitches
+ * are multiples of 8 elements (<= 4 194 296) and whose rows are whole multiples of 8 elements go straight into LDS.  padded, bit 0 for A, bit 1 for B: the rows may
+ * be read up to the next multiple of 8 elements, and are 0 there where they run along the contraction (dm_act8_mask_rows without bits
+ * makes such a copy).  Few output tiles: the contraction is split and the parts (workspace, dm_act8_gemm_workspace_bytes of the same arguments)
+ * are added in order; results depend on shapes, alignments and values alone.
  *   dm_act8_mask_rows  out (rows, ldo), ldo % 8 == 0: x where its sign bit is set (all of x without bits), 0 elsewhere and
  *                      behind the width */
-size_t dm_act8_gemm_workspace_bytes(int form, int dtype, int M, int N, int K);
-int dm_act8_gemm(int form, int dtype, const void *A, long long lda, const void *B, long long ldb, const uint8_t *exps /*form 2*/,
+size_t dm_act8_gemm_workspace_bytes(int form, int dtype, const void *A, long long lda, const void *B, long long ldb, int padded, int M, int N,
+                                    int K);
+int dm_act8_gemm(int form, int dtype, const void *A, long long lda, const void *B, long long ldb, int padded, const uint8_t *exps /*form 2*/,
                  const void *bias /*or NULL*/, int relu, int M, int N, int K, void *C, uint32_t *sign_bits /*or NULL*/,
                  void *rowsum /*or NULL*/, void *workspace, size_t workspace_bytes, dm_stream_t stream);
 int dm_act8_mask_rows(const void *x, int dtype, long long rows, int width, long long ld, const uint32_t *sign_bits /*or NULL*/,
