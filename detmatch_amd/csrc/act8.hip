@@ -38,7 +38,7 @@ __global__ __launch_bounds__(A8_BLOCK) void act8_unpack_kernel(const uint8_t *__
   for (long long r = (long long)blockIdx.x * rpb + ty; r < rows; r += (long long)gridDim.x * rpb) {
     for (int c = tx; c < chunks; c += tpr) {
       const uint2 u = *(const uint2 *)(codes + ((size_t)r * groups * ACT8_GROUP + 8 * c));
-      const int e = (int)exps[(size_t)r * groups + (c >> 2)] - 127;
+      const uint32_t e = exps[(size_t)r * groups + (c >> 2)];
       float v[8];
       act8_decode4(u.x, e, v);
       act8_decode4(u.y, e, v + 4);

@@ -47,12 +47,12 @@ __device__ __forceinline__ uint32_t act8_encode4_fast(float a, float b, float c,
 
 __device__ __forceinline__ float act8_limit(int e) { return e >= 120 ? 240.f : 448.f; }
 
-// four values code * 2^e; the scale is applied in two exact halves, so that e = -127 needs no subnormal factor
-__device__ __forceinline__ void act8_decode4(uint32_t u, int e, float *v) {
+// four values code * 2^e, eb = e + 127 (2^-127 is a subnormal number).  (Converting and multiplying: with the converting instructions that take a
+// scale the backward pass of the norms took 496 us in place of 343 at 32 768 x 4 096 bf16.)
+__device__ __forceinline__ void act8_decode4(uint32_t u, uint32_t eb, float *v) {
   const act8_f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)u, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)u, true);
-  const int h = e >> 1;
-  const float s0 = act8_2exp(h), s1 = act8_2exp(e - h);
-  v[0] = lo[0] * s0 * s1, v[1] = lo[1] * s0 * s1, v[2] = hi[0] * s0 * s1, v[3] = hi[1] * s0 * s1;
+  const float s = __uint_as_float(eb ? eb << 23 : 0x00400000u);
+  v[0] = lo[0] * s, v[1] = lo[1] * s, v[2] = hi[0] * s, v[3] = hi[1] * s;
 }
 
 // ---- 8 consecutive elements of a row, any element type --------------------------------------------------------------

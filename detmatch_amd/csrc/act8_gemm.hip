@@ -81,7 +81,7 @@ __device__ __forceinline__ uint2 deq4(uint32_t u, uint32_t eb) {
   if constexpr (T == ACT8_F16) {
     if (eb >= 127 + 8) {                        // 256 * 2^8 is the one value that fp16 does not have: saturate
       float v[4];
-      act8_decode4(u, (int)eb - 127, v);
+      act8_decode4(u, eb, v);
       union { uint2 w; _Float16 h[4]; } r;
 #pragma unroll
       for (int k = 0; k < 4; ++k) r.h[k] = (_Float16)(v[k] != v[k] ? v[k] : fminf(fmaxf(v[k], -65504.f), 65504.f));

@@ -16,115 +16,11 @@
 // is read once and the two norms of a row follow one another without a second pass.  Bound by memory.
 // Sums over rows: a thread adds its channels over the rows that its team walks, a workgroup's teams are added in LDS, the
 // workgroups' sums go to a workspace and a second kernel adds them in order (no atomics).
-#include "act8_codec.h"
+#include "block_norm.h"
+
+using namespace dm_bn;
 
 namespace {
-
-struct BnArgs {
-  const void *x, *f, *gate, *post_w, *post_b, *pre_w, *pre_b, *scale, *gy, *gh;   // scale: a device number, or NULL: scale_host
-  void *y, *h, *dx, *df, *dgate;
-  const void *y_in;                              // backward: y (exact) ...
-  uint8_t *f_codes, *f_exps, *y_codes, *y_exps;  // ... or codes of f and y
-  float *f_mean, *f_rstd, *y_mean, *y_rstd;      // statistics (rows); means only for the layer norm
-  float *part;                                   // backward: sums per workgroup [set][blocks][C], then [blocks] of the scale's
-  long long ldx, ldf, ldg, ldgy, ldgh;
-  uint32_t rows, each, groups;                   // groups of `each` rows
-  float eps, scale_host, inv_c;
-  int C, T, act, post, w32, s32, by_unit, n_blocks, sets;   // sets: which sums over rows are wanted, a bit each
-};
-
-enum { ACT_NONE = 0, ACT_SIGMOID = 1, ACT_TANH = 2 };
-// sums over rows, in the order of the workspace
-enum { SET_PRE_W = 0, SET_PRE_B = 1, SET_POST_W = 2, SET_POST_B = 3, SET_GATE = 4, SETS = 5 };
-
-__device__ __forceinline__ float act_of(int act, float z) {
-  if (act == ACT_SIGMOID) return __builtin_amdgcn_rcpf(1.f + __expf(-z));
-  if (act == ACT_TANH) return tanhf(z);
-  return z;
-}
-
-__device__ __forceinline__ float act_slope(int act, float g) {      // from the activated value
-  return act == ACT_SIGMOID ? g * (1.f - g) : act == ACT_TANH ? 1.f - g * g : 1.f;
-}
-
-__device__ __forceinline__ float rsqrt_of(float v) {                 // (the instruction takes no subnormal numbers)
-  return v < 1e-30f ? __builtin_amdgcn_rsqf(v * 0x1p64f) * 0x1p32f : __builtin_amdgcn_rsqf(v);
-}
-
-// sums of NV numbers over a team: lane exchanges inside a wave (every lane ends with the same sum), LDS between waves.  `red` holds two sets of
-// partial sums in turn, so one barrier a call is enough: a set is written again only after the barrier of the call in between.
-template <int NV>
-__device__ __forceinline__ void team_sum(float (&v)[NV], int T, float *red, int &turn) {
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    v[i] += act8_dpp<ACT8_DPP_XOR1>(v[i]);
-    v[i] += act8_dpp<ACT8_DPP_XOR2>(v[i]);
-    v[i] += act8_dpp<ACT8_DPP_HALF_MIRROR>(v[i]);
-    if (T >= 16) v[i] += act8_dpp<ACT8_DPP_MIRROR>(v[i]);
-    if (T >= 32) {
-      const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]), __float_as_uint(v[i]), false, false);
-      v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    }
-    if (T >= 64) {
-      const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(v[i]), false, false);
-      v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    }
-  }
-  if (T > 64) {
-    float *r = red + turn * 32;
-    turn ^= 1;
-    const int wave = threadIdx.x >> 6, per = T >> 6;
-    if ((threadIdx.x & 63) == 0) {
-#pragma unroll
-      for (int i = 0; i < NV; ++i) r[wave * NV + i] = v[i];
-    }
-    __syncthreads();
-    const int w0 = wave & ~(per - 1);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) v[i] = 0.f;
-    for (int w = 0; w < per; ++w) {
-#pragma unroll
-      for (int i = 0; i < NV; ++i) v[i] += r[(w0 + w) * NV + i];
-    }
-  }
-}
-
-template <int T>
-__device__ __forceinline__ void load_param(const BnArgs &a, const void *p, int c, float *v, float absent) {
-  if (!p) {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = absent;
-  } else if (a.w32) act8_load8<ACT8_F32>(p, c, a.C - c, v);
-  else act8_load8<T>(p, c, a.C - c, v);
-}
-
-template <int T>
-__device__ __forceinline__ float load_scale(const BnArgs &a) {
-  if (!a.scale) return a.scale_host;
-  return a.s32 ? *(const float *)a.scale : act8_get<T>(a.scale, 0);
-}
-
-// 8 codes of a row and their exponent, in the place of the 8 elements they stand for
-template <int T>
-__device__ __forceinline__ Act8Raw<T> load_codes(const uint8_t *codes, const uint8_t *exps, size_t row, int groups, int c, int n) {
-  Act8Raw<T> r;
-  r.w[0] = act8_u32x4{0u, 0u, 127u, 0u};
-  if (n > 0) {
-    const uint2 u = *(const uint2 *)(codes + (row * groups * ACT8_GROUP + c));
-    r.w[0].x = u.x, r.w[0].y = u.y, r.w[0].z = exps[row * groups + c / ACT8_GROUP];
-  }
-  return r;
-}
-
-template <int T>
-__device__ __forceinline__ void unraw_codes(const Act8Raw<T> &r, float *v) {
-  const int e = (int)r.w[0].z - 127;
-  act8_decode4(r.w[0].x, e, v), act8_decode4(r.w[0].y, e, v + 4);
-  if constexpr (T == ACT8_F16) {                     // (the other types hold every code exactly)
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = v[k] != v[k] ? v[k] : (float)(_Float16)fminf(fmaxf(v[k], -65504.f), 65504.f);
-  }
-}
 
 __device__ __forceinline__ void store_codes8(const float *v, uint8_t *codes, uint8_t *exps, size_t row, int groups, int c, bool live) {
   int e;
@@ -165,10 +61,10 @@ __device__ __forceinline__ void row_stats(const BnArgs &a, const float (&v)[NCH]
 }
 
 // A workgroup's teams walk the rows with the grid's stride.  The next row's operands are under way while this one is computed.
-template <int T, bool LAYER, int NCH, int BLOCK>
+template <int T, bool LAYER, int NCH, int BLOCK, bool WAVES>
 __global__ __launch_bounds__(BLOCK, NCH == 1 ? 4 : 2) void block_norm_fwd_kernel(BnArgs a) {
   __shared__ float red[64];
-  const int tx = threadIdx.x & (a.T - 1), team = threadIdx.x / a.T, teams = BLOCK / a.T, groups8 = (a.C + 31) / 32;
+  const int tx = threadIdx.x & (a.T - 1), team = team_of<WAVES>(a.T), teams = BLOCK / a.T, groups8 = (a.C + 31) / 32;
   int turn = 0;
   const float scale = load_scale<T>(a);
   const bool has_f = a.f != nullptr, gate_each = a.gate && a.groups > 1;
@@ -277,231 +173,6 @@ __global__ __launch_bounds__(BLOCK, NCH == 1 ? 4 : 2) void block_norm_fwd_kernel
   }
 }
 
-// A team walks rows team, team + teams, ... of one group of rows (blockIdx.y) that share their gates, or, where there are many
-// groups, whole groups one after another (by_unit); `each` rows have one row of gates.
-template <int T, bool LAYER, int NCH, int BLOCK>
-__global__ __launch_bounds__(BLOCK) void block_norm_bwd_kernel(BnArgs a) {
-  __shared__ float red[64];
-  __shared__ float sums[BLOCK <= 512 ? BLOCK * 8 : 1];
-  const int tx = threadIdx.x & (a.T - 1), team = threadIdx.x / a.T, teams = BLOCK / a.T, groups8 = (a.C + 31) / 32;
-  int turn = 0;
-  const float scale = load_scale<T>(a);
-  const bool has_f = a.f || a.f_codes, has_h = a.gh != nullptr;
-  float acc[SETS][NCH][8], dscale = 0.f;
-  float post_w[NCH][8], post_b[LAYER ? NCH : 1][8], pre_w[NCH][8], g[NCH][8];
-#pragma unroll
-  for (int n = 0; n < NCH; ++n) {
-    const int c = 8 * (tx + n * a.T);
-    load_param<T>(a, a.post_w, c, post_w[n], 1.f), load_param<T>(a, a.pre_w, c, pre_w[n], 1.f);
-    if constexpr (LAYER) load_param<T>(a, a.post_b, c, post_b[n], 0.f);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      g[n][k] = 1.f;
-#pragma unroll
-      for (int s = 0; s < SETS; ++s) acc[s][n][k] = 0.f;
-    }
-  }
-  const uint32_t stride = gridDim.x * teams, first = blockIdx.x * teams + team;
-  const uint32_t trips = a.by_unit ? (a.groups + stride - 1) / stride * a.each : (a.each + stride - 1) / stride;
-  struct In {
-    Act8Raw<T> gh[NCH], gy[NCH], y[NCH], f[NCH], g[NCH];
-    float y_mean, y_rstd, f_mean, f_rstd;
-    uint32_t row, unit;
-    bool live, last;              // last: the group's last row
-  } next;
-  uint32_t unit = a.by_unit ? first : blockIdx.y, in_unit = a.by_unit ? 0 : first;
-  auto fetch = [&]() {
-    next.live = unit < a.groups && in_unit < a.each;
-    next.row = unit * a.each + in_unit, next.unit = unit;
-    next.last = a.by_unit && in_unit + 1 == a.each;
-    const size_t row = next.row;
-    next.y_mean = next.y_rstd = next.f_mean = next.f_rstd = 0.f;
-    if (next.live) {
-      if (has_h) {
-        next.y_rstd = a.y_rstd[row];
-        if (LAYER) next.y_mean = a.y_mean[row];
-      }
-      if (has_f && a.post) {
-        next.f_rstd = a.f_rstd[row];
-        if (LAYER) next.f_mean = a.f_mean[row];
-      }
-    }
-#pragma unroll
-    for (int n = 0; n < NCH; ++n) {
-      const int c = 8 * (tx + n * a.T), left = next.live ? a.C - c : 0;
-      if (has_h) {
-        next.gh[n] = act8_load_raw<T>(a.gh, row * a.ldgh + c, left);
-        if (a.y_codes) next.y[n] = load_codes<T>(a.y_codes, a.y_exps, row, groups8, c, left);
-        else next.y[n] = act8_load_raw<T>(a.y_in, row * a.ldx + c, left);
-      }
-      if (a.gy) next.gy[n] = act8_load_raw<T>(a.gy, row * a.ldgy + c, left);
-      if (has_f) {
-        if (a.f_codes) next.f[n] = load_codes<T>(a.f_codes, a.f_exps, row, groups8, c, left);
-        else next.f[n] = act8_load_raw<T>(a.f, row * a.ldf + c, left);
-        if (a.gate) next.g[n] = act8_load_raw<T>(a.gate, (size_t)unit * a.ldg + c, left);
-      }
-    }
-    if (!a.by_unit) in_unit += stride;
-    else if (++in_unit == a.each) in_unit = 0, unit += stride;
-  };
-  if (trips) fetch();
-  for (uint32_t i = 0; i < trips; ++i) {
-    const In in = next;
-    if (i + 1 < trips) fetch();
-    float dy[NCH][8];
-#pragma unroll
-    for (int n = 0; n < NCH; ++n) {
-      if (a.gy) act8_unraw<T>(in.gy[n], dy[n]);
-      else
-#pragma unroll
-        for (int k = 0; k < 8; ++k) dy[n][k] = 0.f;
-    }
-    // (channels behind the width, and rows of a team without one: gradients are 0 there, and what multiplies them is finite)
-    if (has_h) {
-      float hat[NCH][8], d[NCH][8], s[2] = {0.f, 0.f};
-#pragma unroll
-      for (int n = 0; n < NCH; ++n) {
-        act8_unraw<T>(in.gh[n], d[n]);
-        if (a.y_codes) unraw_codes<T>(in.y[n], hat[n]);
-        else act8_unraw<T>(in.y[n], hat[n]);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          if (LAYER) hat[n][k] -= in.y_mean;
-          hat[n][k] *= in.y_rstd;
-          acc[SET_PRE_W][n][k] = fmaf(d[n][k], hat[n][k], acc[SET_PRE_W][n][k]);
-          if (LAYER) acc[SET_PRE_B][n][k] += d[n][k];
-          d[n][k] *= pre_w[n][k];
-          s[0] = fmaf(d[n][k], hat[n][k], s[0]);
-          if (LAYER) s[1] += d[n][k];
-        }
-      }
-      if constexpr (LAYER) team_sum<2>(s, a.T, red, turn);
-      else {
-        float one[1] = {s[0]};
-        team_sum<1>(one, a.T, red, turn);
-        s[0] = one[0];
-      }
-      const float m0 = s[0] * a.inv_c, m1 = s[1] * a.inv_c;
-#pragma unroll
-      for (int n = 0; n < NCH; ++n)
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          if (LAYER) d[n][k] -= m1;
-          dy[n][k] = fmaf(in.y_rstd, fmaf(-hat[n][k], m0, d[n][k]), dy[n][k]);
-        }
-    }
-#pragma unroll
-    for (int n = 0; n < NCH; ++n) {
-      const int c = 8 * (tx + n * a.T);
-      if (in.live && a.dx) act8_store8<T>(a.dx, (size_t)in.row * a.C + c, a.C - c, dy[n]);
-    }
-    if (has_f) {
-      float hat[NCH][8], s[2] = {0.f, 0.f};
-#pragma unroll
-      for (int n = 0; n < NCH; ++n) {
-        const int c = 8 * (tx + n * a.T);
-        if (c + 8 > a.C) {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) dy[n][k] = c + k < a.C ? dy[n][k] : 0.f;
-        }
-        if (a.f_codes) unraw_codes<T>(in.f[n], hat[n]);
-        else act8_unraw<T>(in.f[n], hat[n]);
-        if (a.gate) {
-          act8_unraw<T>(in.g[n], g[n]);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) g[n][k] = act_of(a.act, g[n][k]);
-        }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          float u = hat[n][k], t = dy[n][k];
-          if (a.post) {
-            if (LAYER) hat[n][k] -= in.f_mean;
-            hat[n][k] *= in.f_rstd;
-            u = LAYER ? fmaf(hat[n][k], post_w[n][k], post_b[n][k]) : hat[n][k] * post_w[n][k];
-          }
-          const float tu = t * u;
-          dscale = fmaf(tu, g[n][k], dscale);
-          if (a.gate) acc[SET_GATE][n][k] += tu;
-          t *= g[n][k];
-          if (a.post) {
-            acc[SET_POST_W][n][k] = fmaf(t, hat[n][k], acc[SET_POST_W][n][k]);
-            if (LAYER) acc[SET_POST_B][n][k] += t;
-            t *= post_w[n][k];
-            s[0] = fmaf(t, hat[n][k], s[0]);
-            if (LAYER) s[1] += t;
-          }
-          dy[n][k] = t;
-        }
-      }
-      float r = scale;
-      if (a.post) {
-        if constexpr (LAYER) team_sum<2>(s, a.T, red, turn);
-        else {
-          float one[1] = {s[0]};
-          team_sum<1>(one, a.T, red, turn);
-          s[0] = one[0];
-        }
-        const float m0 = s[0] * a.inv_c, m1 = s[1] * a.inv_c;
-        r *= in.f_rstd;
-#pragma unroll
-        for (int n = 0; n < NCH; ++n)
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            if (LAYER) dy[n][k] -= m1;
-            dy[n][k] = fmaf(-hat[n][k], m0, dy[n][k]);
-          }
-      }
-#pragma unroll
-      for (int n = 0; n < NCH; ++n) {
-        const int c = 8 * (tx + n * a.T);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) dy[n][k] *= r;
-        if (in.live && a.df) act8_store8<T>(a.df, (size_t)in.row * a.C + c, a.C - c, dy[n]);
-        if (in.last && a.gate) {                     // this group of rows is done: its gates' gradient is complete
-          float v[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            v[k] = acc[SET_GATE][n][k] * scale * act_slope(a.act, g[n][k]);
-            acc[SET_GATE][n][k] = 0.f;
-          }
-          if (in.live && a.dgate) act8_store8<T>(a.dgate, (size_t)in.unit * a.C + c, a.C - c, v);
-        }
-      }
-    }
-  }
-  // this workgroup's sums; the residual scale, the same for all, is multiplied on when they are added up
-  const size_t block = (size_t)blockIdx.y * gridDim.x + blockIdx.x;
-  if (BLOCK <= 512 && teams > 1) {
-#pragma unroll
-    for (int s = 0; s < SETS; ++s) {
-      if (!((a.sets >> s) & 1)) continue;
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < 8; ++k) sums[threadIdx.x * 8 + k] = acc[s][0][k];
-      __syncthreads();
-      for (int c = threadIdx.x; c < a.C; c += BLOCK) {
-        float v = 0.f;
-        for (int t = 0; t < teams; ++t) v += sums[t * a.T * 8 + c];
-        a.part[((size_t)s * a.n_blocks + block) * a.C + c] = v;
-      }
-    }
-  } else {
-#pragma unroll
-    for (int s = 0; s < SETS; ++s) {
-      if (!((a.sets >> s) & 1)) continue;
-#pragma unroll
-      for (int n = 0; n < NCH; ++n) {
-        const int c = 8 * (tx + n * a.T);
-        act8_store8<ACT8_F32>(a.part, ((size_t)s * a.n_blocks + block) * a.C + c, a.C - c, acc[s][n]);
-      }
-    }
-  }
-  float ds[1] = {dscale};
-  __syncthreads();
-  team_sum<1>(ds, BLOCK, red, turn);
-  if (threadIdx.x == 0) a.part[(size_t)SETS * a.n_blocks * a.C + block] = ds[0];
-}
-
 struct SumArgs {
   const float *part;
   void *out[SETS], *dscale;
@@ -559,63 +230,23 @@ __global__ __launch_bounds__(1024) void block_norm_sum_kernel(SumArgs a) {
   else act8_put<T>(a.out[set], c, v);
 }
 
-struct BnPlan {
-  int T, nch, block;
-};
-
-bool bn_plan(int C, BnPlan *p) {
-  const int chunks = dm_ceil_div(C, 8);
-  int t = 8;
-  while (t < chunks && t < 512) t <<= 1;
-  if (chunks > 2 * t) t <<= 1;
-  p->T = t;
-  p->nch = dm_ceil_div(chunks, t);
-  p->block = t <= 512 ? 512 : t;
-  return p->nch <= 2;
-}
-
-// workgroups of the backward kernel: x for one group, y groups (by_unit: all groups in x)
-struct BnGrid {
-  int x, y, by_unit;
-};
-
-BnGrid bn_grid(const BnPlan &p, long long rows, long long groups) {
-  const int teams = p.block / p.T, most = 512;      // two workgroups a compute unit: each of them leaves sums behind
-  BnGrid g;
-  g.by_unit = groups > 64;
-  const long long units = g.by_unit ? groups : rows / (groups > 0 ? groups : 1);
-  g.y = g.by_unit || groups < 1 ? 1 : (int)groups;
-  long long x = (units + teams - 1) / teams, cap = most / g.y > 0 ? most / g.y : 1;
-  g.x = (int)(x < cap ? x : cap);
-  return g;
-}
-
 template <int T, bool LAYER>
 int launch_fwd(const BnArgs &a, const BnPlan &p, hipStream_t st) {
   const int teams = p.block / p.T;
   const uint32_t blocks = (a.rows + teams - 1) / teams, most = 1024;   // (as many as are resident at once, and parameters are read once)
   const unsigned grid = blocks < most ? blocks : most;
-  if (p.block == 512 && p.nch == 1) block_norm_fwd_kernel<T, LAYER, 1, 512><<<grid, 512, 0, st>>>(a);
-  else if (p.block == 512) block_norm_fwd_kernel<T, LAYER, 2, 512><<<grid, 512, 0, st>>>(a);
-  else block_norm_fwd_kernel<T, LAYER, 2, 1024><<<grid, 1024, 0, st>>>(a);
-  DM_CHECK_LAUNCH();
-  return DM_OK;
-}
-
-template <int T, bool LAYER>
-int launch_bwd(const BnArgs &a, const BnPlan &p, const BnGrid &g, hipStream_t st) {
-  const dim3 grid(g.x, g.y);
-  if (p.block == 512 && p.nch == 1) block_norm_bwd_kernel<T, LAYER, 1, 512><<<grid, 512, 0, st>>>(a);
-  else if (p.block == 512) block_norm_bwd_kernel<T, LAYER, 2, 512><<<grid, 512, 0, st>>>(a);
-  else block_norm_bwd_kernel<T, LAYER, 2, 1024><<<grid, 1024, 0, st>>>(a);
+  if (p.T < 64) block_norm_fwd_kernel<T, LAYER, 1, 512, false><<<grid, 512, 0, st>>>(a);
+  else if (p.block == 512 && p.nch == 1) block_norm_fwd_kernel<T, LAYER, 1, 512, true><<<grid, 512, 0, st>>>(a);
+  else if (p.block == 512) block_norm_fwd_kernel<T, LAYER, 2, 512, true><<<grid, 512, 0, st>>>(a);
+  else block_norm_fwd_kernel<T, LAYER, 2, 1024, true><<<grid, 1024, 0, st>>>(a);
   DM_CHECK_LAUNCH();
   return DM_OK;
 }
 
 // what forward and backward have in common; returns a DM_ERR_* code
-int fill(BnArgs *a, const dm_block_norm *q, BnPlan *p) {
+int fill(BnArgs *a, const dm_block_norm *q, bool backward, BnPlan *p) {
   if (!q || q->dtype < ACT8_F32 || q->dtype > ACT8_F16 || q->rows < 0 || q->rows > 0x7ffffc00 || q->width <= 0) return DM_ERR_INVALID_ARG;
-  if (!bn_plan(q->width, p)) return DM_ERR_UNSUPPORTED;
+  if (!bn_plan(q->width, backward, p)) return DM_ERR_UNSUPPORTED;
   if (q->gate_act < ACT_NONE || q->gate_act > ACT_TANH || q->groups < 0 || (q->gate ? q->groups < 1 || q->rows % q->groups : q->groups != 0))
     return DM_ERR_INVALID_ARG;
   if (q->gate && q->ld_gate < q->width && q->groups > 1) return DM_ERR_INVALID_ARG;
@@ -639,7 +270,7 @@ extern "C" int dm_block_norm_forward(const dm_block_norm *q, const void *x, long
                                      dm_stream_t stream) {
   BnArgs a = {};
   BnPlan p;
-  const int rc = fill(&a, q, &p);
+  const int rc = fill(&a, q, false, &p);
   if (rc != DM_OK) return rc;
   if (q->rows == 0) return DM_OK;
   if (!x || ldx < q->width || (f && (!y || ldf < q->width)) || (!f && (!h || y || q->gate)) || (q->f_codes && !f)) return DM_ERR_INVALID_ARG;
@@ -654,7 +285,7 @@ extern "C" int dm_block_norm_forward(const dm_block_norm *q, const void *x, long
 
 extern "C" size_t dm_block_norm_workspace_bytes(long long rows, int width, long long groups) {
   BnPlan p;
-  if (rows <= 0 || width <= 0 || groups < 0 || !bn_plan(width, &p)) return 0;
+  if (rows <= 0 || width <= 0 || groups < 0 || !bn_plan(width, true, &p)) return 0;
   const BnGrid g = bn_grid(p, rows, groups);
   return dm_align((size_t)g.x * g.y * ((size_t)SETS * width + 1) * sizeof(float));
 }
@@ -665,11 +296,12 @@ extern "C" int dm_block_norm_backward(const dm_block_norm *q, const void *gy, lo
                                       dm_stream_t stream) {
   BnArgs a = {};
   BnPlan p;
-  const int rc = fill(&a, q, &p);
+  const int rc = fill(&a, q, true, &p);
   if (rc != DM_OK) return rc;
   if (q->rows == 0) return DM_ERR_INVALID_ARG;                     // (there is nothing to sum: the caller writes the zeros)
   const bool layer = q->layer != 0, has_f = f || q->f_codes;
   if ((gy && ldgy < q->width) || (gh && ldgh < q->width) || (!gy && !gh)) return DM_ERR_INVALID_ARG;
+  if ((q->f_codes || q->y_codes) && ((has_f && !q->f_codes) || (gh && !q->y_codes))) return DM_ERR_INVALID_ARG;
   if (gh && (!a.y_rstd || (layer && !a.y_mean) || !(y || q->y_codes) || (y && ldy < q->width))) return DM_ERR_INVALID_ARG;
   if (has_f && q->post && (!a.f_rstd || (layer && !a.f_mean))) return DM_ERR_INVALID_ARG;
   if ((f && ldf < q->width) || (!has_f && (df || dgate || dpost_w || dpost_b || dscale))) return DM_ERR_INVALID_ARG;
@@ -683,10 +315,7 @@ extern "C" int dm_block_norm_backward(const dm_block_norm *q, const void *gy, lo
   a.sets = (dpre_w ? 1 << SET_PRE_W : 0) | (dpre_b ? 1 << SET_PRE_B : 0) | (dpost_w ? 1 << SET_POST_W : 0) | (dpost_b ? 1 << SET_POST_B : 0) |
            (dgate && !g.by_unit ? 1 << SET_GATE : 0);
   hipStream_t st = (hipStream_t)stream;
-  int e;
-  if (dt == ACT8_F32) e = layer ? launch_bwd<ACT8_F32, true>(a, p, g, st) : launch_bwd<ACT8_F32, false>(a, p, g, st);
-  else if (dt == ACT8_BF16) e = layer ? launch_bwd<ACT8_BF16, true>(a, p, g, st) : launch_bwd<ACT8_BF16, false>(a, p, g, st);
-  else e = layer ? launch_bwd<ACT8_F16, true>(a, p, g, st) : launch_bwd<ACT8_F16, false>(a, p, g, st);
+  const int e = dm_block_norm_launch_backward(dt, layer, a, p, g, st);
   if (e != DM_OK) return e;
   SumArgs s = {};
   s.part = a.part, s.dscale = dscale, s.gate = q->gate, s.ldg = q->ld_gate, s.C = q->width, s.act = q->gate_act, s.n_blocks = a.n_blocks;
