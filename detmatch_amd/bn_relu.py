@@ -9,7 +9,7 @@ import torch
 import torch.nn.functional as F
 from torch.autograd import Function
 
-from . import _lib
+from . import _lib, act8
 
 
 class _BNReLURows(Function):
@@ -218,21 +218,24 @@ def bn_relu_rows(x, bn, relu=True):
     return F.relu(y, inplace=True) if relu else y
 
 
-def _linear_rows(x, m):
+def _linear_rows(x, m, keep8=False):
     # (the RoI head's 27648 -> 256 layer was also tried as a split-K 1x1 convolution on conv2d.hip:
     # 290 us forward + backward against 212 us of the BLAS kernels torch picks — kept on BLAS)
     # (vendor GEMM: only ever inside _lib.blas_turn — one Stream-K kernel at a time)
-    w = m.weight
-    return _lib.blas_linear(x, w.squeeze(-1) if w.dim() == 3 else w, m.bias)
+    w = m.weight.squeeze(-1) if m.weight.dim() == 3 else m.weight
+    return act8.linear(x, w, m.bias) if keep8 else _lib.blas_linear(x, w, m.bias)
 
 
-def fc_rows(seq, x):
+def fc_rows(seq, x, keep8=False):
     """An nn.Sequential of Linear / Conv1d(kernel 1) + BatchNorm1d + ReLU (+ Dropout) layers — the FC
     stacks of the PV-RCNN heads (pvrcnn_head.py:25-52 builds them from Conv1d on (N, C, 1) tensors,
     point_head_template.py:34-47 and voxel_set_abstraction.py:107-111 from Linear) — evaluated on the
     (N, C) row view with the same parameters and state-dict keys: a plain GEMM per layer and the
-    fused BatchNorm+ReLU row kernel instead of one convolution / batch-norm library call per layer."""
+    fused BatchNorm+ReLU row kernel instead of one convolution / batch-norm library call per layer.
+    Residual blocks (residual_rows.ResidualRows) may stand among the layers.  keep8: the layers keep their inputs for the
+    backward pass in 8 bits (act8.linear)."""
     import torch.nn as nn
+    from .residual_rows import ResidualRows
     mods = list(seq)
     i = 0
     while i < len(mods):
@@ -240,7 +243,7 @@ def fc_rows(seq, x):
         if isinstance(m, (nn.Conv1d, nn.Linear)):
             if isinstance(m, nn.Conv1d):
                 assert m.kernel_size == (1,) and m.stride == (1,) and m.padding == (0,) and m.groups == 1
-            x = _linear_rows(x, m)
+            x = _linear_rows(x, m, keep8)
         elif isinstance(m, nn.BatchNorm1d):
             relu = i + 1 < len(mods) and isinstance(mods[i + 1], nn.ReLU)
             x = bn_relu_rows(x, m, relu=relu)
@@ -249,6 +252,8 @@ def fc_rows(seq, x):
             x = F.dropout(x, m.p, m.training, False)
         elif isinstance(m, nn.ReLU):
             x = F.relu(x)
+        elif isinstance(m, ResidualRows):
+            x = m(x)
         else:
             raise TypeError('unexpected layer %s in an FC stack' % type(m).__name__)
         i += 1

@@ -16,7 +16,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from .. import _lib, dense_conv
+from .. import _lib, act8, dense_conv
 from ..devconst import const
 from ..mm3d.base_detector import DetectorStepMixin
 from ..mm3d.losses import bbox_overlaps
@@ -454,10 +454,12 @@ class RPNHead(nn.Module):
 
 # ------------------------------------------------------------------ RoI head
 class Shared2FCBBoxHead(nn.Module):
+    """keep8: the FC layers keep their inputs for the backward pass in 8 bits and their ReLU masks in one bit (act8.linear)."""
 
     def __init__(self, in_channels=256, fc_out_channels=1024, roi_feat_size=7, num_classes=80,
-                 bbox_coder=None, reg_class_agnostic=False, loss_cls=None, loss_bbox=None, **kwargs):
+                 bbox_coder=None, reg_class_agnostic=False, loss_cls=None, loss_bbox=None, keep8=False, **kwargs):
         super().__init__()
+        self.keep8 = bool(keep8)
         self.num_classes = num_classes
         self.reg_class_agnostic = reg_class_agnostic
         bc = dict(bbox_coder)
@@ -479,11 +481,11 @@ class Shared2FCBBoxHead(nn.Module):
 
     def forward(self, x):
         x = x.flatten(1)
+        linear = act8.linear if self.keep8 else _lib.blas_linear
         # (vendor GEMMs: only ever inside _lib.blas_turn — one Stream-K kernel at a time)
         for fc in self.shared_fcs:
-            x = _lib.blas_linear(x, fc.weight, fc.bias, relu=True)
-        return _lib.blas_linear(x, self.fc_cls.weight, self.fc_cls.bias), \
-            _lib.blas_linear(x, self.fc_reg.weight, self.fc_reg.bias)
+            x = linear(x, fc.weight, fc.bias, relu=True)
+        return linear(x, self.fc_cls.weight, self.fc_cls.bias), linear(x, self.fc_reg.weight, self.fc_reg.bias)
 
     def loss(self, cls_score, bbox_pred, labels, label_weights, bbox_targets, bbox_weights, fused=None):
         """mmdet BBoxHead.loss: cls avg_factor = #(label_weights > 0); box loss over positives of

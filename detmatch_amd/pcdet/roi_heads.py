@@ -21,6 +21,7 @@ from ..devconst import const
 from .. import pointnet2_stack as pn2
 from . import utils as U
 from ..bn_relu import fc_rows
+from ..residual_rows import ResidualRows
 from ..fused import on as fused_on
 from .dense_heads import valid_gt_mask
 from .pfe import batch_row_counts
@@ -280,7 +281,11 @@ class _RoiDecode(torch.autograd.Function):
 
 
 class PVRCNNHead(nn.Module):
-    """roi_head_template.py:11-263 + pvrcnn_head.py:8-201."""
+    """roi_head_template.py:11-263 + pvrcnn_head.py:8-201.
+
+    Two keys of the configuration are this framework's own: KEEP8 (default False): the FC layers keep their inputs for the
+    backward pass in 8 bits (act8.linear); SHARED_RESIDUAL (default: none): the arguments of residual_rows.ResidualRows, `channels`
+    apart, for residual blocks behind SHARED_FC."""
 
     def __init__(self, input_channels, model_cfg, num_class=1, **kwargs):
         super().__init__()
@@ -305,6 +310,9 @@ class PVRCNNHead(nn.Module):
             pre_channel = model_cfg.SHARED_FC[k]
             if k != len(model_cfg.SHARED_FC) - 1 and model_cfg.DP_RATIO > 0:
                 shared.append(nn.Dropout(model_cfg.DP_RATIO))
+        if model_cfg.get('SHARED_RESIDUAL'):
+            shared.append(ResidualRows(pre_channel, **model_cfg.SHARED_RESIDUAL))
+        self.keep8 = bool(model_cfg.get('KEEP8', False))
         self.shared_fc_layer = nn.Sequential(*shared)
         self.cls_layers = self.make_fc_layers(pre_channel, self.num_class, model_cfg.CLS_FC)
         self.reg_layers = self.make_fc_layers(pre_channel, self.box_coder.code_size * self.num_class,
@@ -436,9 +444,9 @@ class PVRCNNHead(nn.Module):
         pooled = self.roi_grid_pool(batch_dict)                           # (B*N, 216, C)
         n_rcnn = pooled.shape[0]
         pooled = pooled.permute(0, 2, 1).contiguous()                    # (B*N, C, 216)
-        shared = fc_rows(self.shared_fc_layer, pooled.view(n_rcnn, -1))
-        rcnn_cls = fc_rows(self.cls_layers, shared)                # (B*N, 1 or num_class)
-        rcnn_reg = fc_rows(self.reg_layers, shared)                # (B*N, code_size * ...)
+        shared = fc_rows(self.shared_fc_layer, pooled.view(n_rcnn, -1), self.keep8)
+        rcnn_cls = fc_rows(self.cls_layers, shared, self.keep8)    # (B*N, 1 or num_class)
+        rcnn_reg = fc_rows(self.reg_layers, shared, self.keep8)    # (B*N, code_size * ...)
         batch_cls_preds, batch_box_preds = self.generate_predicted_boxes(
             batch_dict['batch_size'], batch_dict['rois'], rcnn_cls, rcnn_reg)
         batch_dict['batch_cls_preds'] = batch_cls_preds
