@@ -247,8 +247,8 @@ def linear(x, w, b=None, relu=False):
     """[relu](x w^T + b) for x (..., in), w (out, in), b (out) of one type (float32, bfloat16 or float16), on csrc/act8_gemm.hip.
 
     Kept for the backward pass: pack(x) where w needs a gradient, one bit per output where there is a ReLU, w where x needs a
-    gradient.  gw = g^T unpack(pack(x)), gx = g w, gb = sum of g over rows, g = the gradient behind the ReLU (0 where its output
-    is 0).  x may be overwritten after the call.  Differentiable once."""
+    gradient.  gw = g^T unpack(pack(x)), gx = g w, gb = sum of g over rows, g = the gradient behind the ReLU (0 where its output,
+    as it is stored, is 0).  x may be overwritten after the call.  Differentiable once."""
     if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1]:
         raise ValueError('x (..., in) and w (out, in) are wanted, got %s and %s' % (tuple(x.shape), tuple(w.shape)))
     if b is not None and tuple(b.shape) != (w.shape[0],):

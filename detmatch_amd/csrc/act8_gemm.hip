@@ -30,7 +30,7 @@ struct A8Args {
   const uint8_t *exps;        // form 2: exponents of B's codes, groups per row = ldb / 32
   void *C;
   float *part;                // [splits][M][N] when splits > 1, and behind it [splits][M] row sums
-  uint32_t *bits;             // sign bits of C > 0, (M, ceil(N / 32))
+  uint32_t *bits;             // sign bits of C, (M, ceil(N / 32)): see passes
   void *rowsum;               // form 2: sum over the contraction of A's columns (M)
   int M, N, K;
   long long lda, ldb;
@@ -95,6 +95,12 @@ __device__ __forceinline__ uint2 deq4(uint32_t u, uint32_t eb) {
     const bf16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)u, scale, true);
     return make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
   }
+}
+
+// The ReLU's gradient passes where v, as it is stored, is not <= 0: half the smallest number of the type is rounded to 0 (a nan passes).
+template <int T>
+__device__ __forceinline__ bool passes(float v) {
+  return !(v <= (T == ACT8_F32 ? 0.f : T == ACT8_BF16 ? 0x1p-134f : 0x1p-25f));
 }
 
 // three bf16 pieces of two fp32 values each: the leading 8 bits, the next 8, the last 8 (truncated, so that nothing overflows)
@@ -344,7 +350,7 @@ __device__ __forceinline__ void store_rows(const A8Args &a, const Tile &t, const
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       v[k] += bias[k];
-      if (v[k] > 0.f) word |= 1u << k;
+      if (passes<T>(v[k])) word |= 1u << k;
       if (a.relu) v[k] = v[k] < 0.f ? 0.f : v[k];            // (a nan stays one)
     }
     act8_store8<T>(a.C, (size_t)m * a.N + n, left_n, v);
@@ -739,7 +745,7 @@ __global__ __launch_bounds__(256) void a8_reduce_kernel(A8Args a, int col4, unsi
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     if (a.bias && n + k < a.N) v[k] += act8_get<T>(a.bias, n + k);
-    if (v[k] > 0.f) word |= 1u << ((n & 31) + k);
+    if (passes<T>(v[k])) word |= 1u << ((n & 31) + k);
     if (a.relu) v[k] = v[k] < 0.f ? 0.f : v[k];
   }
   put4<T>(a, m, n, v);

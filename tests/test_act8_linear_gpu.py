@@ -223,3 +223,22 @@ def test_not_a_number_and_infinity_reach_the_outputs(dev):
         assert y[3].isnan().all() and not y[4].isfinite().any() and y[5:].isfinite().all()
         gw, = torch.autograd.grad(y, [w], gy)
         assert gw[:, 5].isnan().all() and gw[:, 6].isnan().all() and gw[:, 7:].isfinite().all()
+
+
+def test_relu_gradient_where_an_output_underflows_or_is_nan(dev):
+    """The mask is that of the stored output: what is rounded to 0 has no gradient, its neighbours and a nan have."""
+    for dtype, unit in ((torch.float16, 2.0 ** -24), (torch.bfloat16, 2.0 ** -133)):
+        b = torch.tensor([unit, -unit, 3 * unit, 0.0, 1.0, float('nan')], dtype=dtype, device=dev)
+        for split in (1, 4096):                # (the second: a split contraction, whose sums are joined by another kernel)
+            # row 0 is b itself; rows 1 and 2 have a product of two small powers on top, half a unit of fp16
+            xx = torch.zeros(3, split, dtype=dtype, device=dev)
+            ww = torch.zeros(6, split, dtype=dtype, device=dev)
+            xx[1, 0], xx[2, 0] = (2.0 ** -12, -2.0 ** -12) if dtype == torch.float16 else (2.0 ** -60, -2.0 ** -60)
+            ww[:, 0] = 2.0 ** -13 if dtype == torch.float16 else 2.0 ** -65
+            leaves = [t.requires_grad_(True) for t in (xx, ww, b.clone())]
+            y = act8.linear(*leaves, relu=True)
+            gy = torch.ones_like(y)
+            gb, = torch.autograd.grad(y, leaves[2:], gy)
+            want = (~(y.detach() <= 0)).double().sum(0)
+            assert torch.equal(gb.double(), want), (dtype, split, gb, want, y)
+            assert bool(y[:, 5].isnan().all()) and float(gb[5]) == 3 and float(gb[1]) <= 1 and float(gb[4]) == 3
