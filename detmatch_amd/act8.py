@@ -121,10 +121,15 @@ def unpack(kept, dtype=None):
     value."""
     if not isinstance(kept, Act8):
         raise TypeError('unpack takes what pack returned, got %s' % type(kept).__name__)
+    width = kept.shape[-1]
+    rows, groups = kept.shape.numel() // width, (width + GROUP - 1) // GROUP
+    for t, shape, name in ((kept.codes, (rows, groups * GROUP), 'codes'), (kept.exps, (rows, groups), 'exps')):
+        if t.dtype != torch.uint8 or t.shape != shape or not t.is_contiguous():
+            raise ValueError('%s: a contiguous uint8 tensor %s is wanted, got %s %s' % (name, shape, t.dtype, tuple(t.shape)))
     out = torch.empty(kept.shape, dtype=kept.dtype if dtype is None else dtype, device=kept.codes.device)
     code = _dtype_code(out, 'dtype')
     with _on(_device_of(kept.codes, kept.exps)):
-        _lib.check(_lib.lib().dm_act8_unpack(_lib.ptr(kept.codes), _lib.ptr(kept.exps), kept.codes.shape[0], kept.shape[-1],
+        _lib.check(_lib.lib().dm_act8_unpack(_lib.ptr(kept.codes), _lib.ptr(kept.exps), rows, width,
                                              _lib.ptr(out), code, _lib.stream()), 'dm_act8_unpack')
     return out
 

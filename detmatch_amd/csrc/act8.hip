@@ -8,7 +8,9 @@ constexpr int A8_BLOCK = 256;
 
 // Rows of `width` elements -> codes (rows, 32 * groups) and exponents (rows, groups).  A thread holds 8 neighbouring
 // elements, 4 threads a group; `tpr` threads (a power of two) walk one row, 256 / tpr rows to a workgroup.
-// Bound by memory: element size in, 1 + 1/32 bytes out.
+// Bound by memory: element size in, 1 + 1/32 bytes out.  8 elements a thread make one 16-byte load (two in fp32), one 8-byte store and a
+// maximum over 4 lanes without LDS.  4 096 x 12 544 bf16: 26 us, 6.0 TB/s (some of x is still in the last cache); with its way back 61 us, 5.1
+// TB/s, the rate of a copy.  1 999 x 12 544 fp32: 22 us.
 template <int T>
 __global__ __launch_bounds__(A8_BLOCK) void act8_pack_kernel(const void *__restrict__ x, long long rows, int width, long long ld,
                                                              int groups, int tpr, uint8_t *__restrict__ codes,
@@ -28,6 +30,7 @@ __global__ __launch_bounds__(A8_BLOCK) void act8_pack_kernel(const void *__restr
   }
 }
 
+// The way back: a multiplication by a power of two, exact but for fp16's range.  Bound by memory; 4 096 x 12 544 bf16: 23 us.
 template <int T>
 __global__ __launch_bounds__(A8_BLOCK) void act8_unpack_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ exps,
                                                                long long rows, int width, int groups, int tpr,

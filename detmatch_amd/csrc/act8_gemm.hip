@@ -418,7 +418,11 @@ __device__ __forceinline__ void store_sum(const A8Args &a, const Tile &t, float 
   else act8_put<T>(a.rowsum, m, v);
 }
 
-// REGS: operands at any address, through registers.  WK groups of WM x WN waves share a tile: each multiplies its part of every step's contraction, and they add up at the end.
+// REGS: operands at any address, through registers.  WK groups of WM x WN waves share a tile: each multiplies its part of every step's
+// contraction, and they add up at the end.
+// Large products are bound by the matrix instructions and the clock that they leave (8 192^3 bf16, forms 0 / 1 / 2: 1 211 / 1 170 / 1 004 TFLOP/s, the
+// library's plain product 1 357 to 1 550; 16 384 x 4 096 x 4 096: 464 / 509 / 558 us = 1 184 / 1 080 / 985).  Form 2 pays for its transposed reads and for
+// the codes' way through registers.  Small ones are bound by the loads' latency over a few steps: 777 x 1 001 x 515 fp16 13 / 14 / 17 us.
 template <int T, int FORM, int WM, int WN, int FM, int FN, int BK, int STAGES, int WK, bool REGS>
 __global__ __launch_bounds__(64 * WM * WN * WK, 2) void a8_gemm16_kernel(A8Args a) {
   constexpr int BM = WM * FM * 32, BN = WN * FN * 32, THREADS = 64 * WM * WN * WK, STAGE = (BM + BN) * BK;
@@ -603,7 +607,8 @@ __global__ __launch_bounds__(64 * WM * WN * WK, 2) void a8_gemm16_kernel(A8Args 
 
 // ---- the fp32 product ----------------------------------------------------------------------------------------------------
 // 128 x 128 tile, 4 waves of 64 x 64, 32 of the contraction at a time; the next step's operands are in registers while this
-// one's planes are multiplied.
+// one's planes are multiplied.  Bound by matrix instructions and the cutting beside them: 1 999 x 12 544 -> 1 024, forms 0 / 1 / 2: 274 / 309 / 206 us,
+// 1 124 / 997 / 747 TFLOP/s of bf16 products = 187 / 166 / 249 of fp32 ones (the library's fp32 product: 152); 256 x 27 648 -> 256: 33 / 30 / 20 us.
 template <int FORM>
 __global__ __launch_bounds__(256, 3) void a8_gemm32_kernel(A8Args a) {
   constexpr int BM = 128, BN = 128, BK = 32, THREADS = 256, FM = 2, FN = 2, PB = FORM == 2 ? 1 : 3;
@@ -756,7 +761,8 @@ __global__ __launch_bounds__(256) void a8_reduce_kernel(A8Args a, int col4, unsi
 }
 
 // ---- a gradient behind a ReLU / rows moved to a 16-byte pitch --------------------------------------------------------------
-// out (rows, ldo) = bits ? (bit set ? x : 0) : x, 0 behind the width; a thread has 8 elements
+// out (rows, ldo) = bits ? (bit set ? x : 0) : x, 0 behind the width; a thread has 8 elements.  Bound by memory: 4 096 x 4 096 bf16 13 us, 5.2 TB/s.
+// (Taking the mask inside the products instead would put the gradient through registers there: the direct path to LDS is worth more.)
 template <int T>
 __global__ __launch_bounds__(256) void a8_mask_kernel(const void *__restrict__ x, long long rows, int width, long long ld,
                                                       const uint32_t *__restrict__ bits, void *__restrict__ out, int ldo) {

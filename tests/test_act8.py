@@ -98,3 +98,13 @@ def test_gemm_entry_checks_its_arguments():
     assert L.dm_act8_gemm_workspace_bytes(0, 1, p, 64, p, 64, 0, 0, 64, 64) == 0
     assert L.dm_act8_mask_rows(p, 1, 4, 12, 12, None, p, 12, None) == bad and L.dm_act8_mask_rows(p, 1, 4, 12, 8, None, p, 16, None) == bad
     assert L.dm_act8_mask_rows(None, 1, 0, 12, 12, None, None, 16, None) == 0
+
+
+def test_unpack_refuses_codes_that_do_not_fit_their_shape():
+    codes, exps = torch.zeros(4, 64, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.uint8)
+    for c, e, shape in ((codes, exps, (4, 65)), (codes, exps, (5, 64)), (codes, exps, (4, 32)), (codes[:, ::2], exps, (4, 32)),
+                        (codes, exps[:, :1], (4, 64)), (codes.int(), exps, (4, 64)), (codes, exps.int(), (4, 64)), (codes[:3], exps, (4, 64))):
+        with pytest.raises(ValueError):
+            act8.unpack(act8.Act8(c, e, shape, torch.float32))
+    with pytest.raises(_lib.DetMatchHipError):
+        act8.unpack(act8.Act8(codes, exps, (2, 2, 40), torch.float32))
