@@ -73,6 +73,7 @@ def test_entry_points_check_their_arguments():
     assert backward(rows=0) == bad and backward(gy=None, gh=None) == bad and backward(y=None) == bad and backward(y_rstd=None) == bad
     assert backward(f_rstd=None) == bad and backward(layer=1) == bad and backward(f=None, dscale=p) == bad and backward(dgate=p) == bad
     assert backward(gh=None, dpre_w=p) == bad and backward(dpost_b=p) == bad and backward(post=0, dpost_w=p) == bad
+    assert backward(f_codes=p, f_exps=p) == bad and backward(y_codes=p, y_exps=p) == bad       # codes of both, or of neither
     assert backward(ws=None) == 2 and backward(nb=16) == 2
     assert L.dm_block_norm_workspace_bytes(0, 16, 0) == 0 and L.dm_block_norm_workspace_bytes(4, 16385, 0) == 0
     assert L.dm_block_norm_workspace_bytes(4, 16, 0) >= 4 * (5 * 16 + 1)

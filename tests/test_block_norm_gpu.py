@@ -15,6 +15,11 @@ TYPES = [torch.float32, torch.bfloat16, torch.float16]
 U = 2.0 ** -24
 
 
+def _requested():
+    """Bytes that are asked for and alive (memory_allocated counts an allocator's blocks, which may be up to 1 MiB larger than asked for)."""
+    return torch.cuda.memory_stats()['requested_bytes.all.current']
+
+
 def _near(got, want, ulps, what):
     v, mag = want
     got = got.detach()
@@ -185,9 +190,9 @@ def test_what_is_kept(dev):
     for t in (x, p['f']):
         t.requires_grad_(True)
     torch.cuda.synchronize()
-    before = torch.cuda.memory_allocated()
+    before = _requested()
     y, h = block_norm.residual_norm(x, keep8=True, **p, **more)
-    held = torch.cuda.memory_allocated() - before - 2 * 2 * rows * width
+    held = _requested() - before - 2 * 2 * rows * width
     assert held <= 2 * rows * width * (1 + 1 / 32) + 4 * 4 * rows + 8192
     with torch.no_grad():
         y2, h2 = block_norm.residual_norm(x, keep8=True, **p, **more)
