@@ -10,6 +10,7 @@ namespace {
 template <int T, bool KEEP8>
 struct Waiting {
   Act8Raw<T> r;
+  template <bool>
   __device__ __forceinline__ void load(const void *p, long long ld, const uint8_t *, const uint8_t *, uint32_t row, uint32_t, int, int c, int n) {
     r = act8_load_raw<T>(p, (size_t)row * ld + c, n);
   }
@@ -20,13 +21,17 @@ template <int T>
 struct Waiting<T, true> {
   uint2 u;
   uint32_t e;
-  // (Behind a row's end and for a team without a row, other codes take the place of zeros: what they are multiplied with is 0.)
+  // Behind a row's end and for a team without a row: zeros, or, CLAMP, other codes (what they are multiplied with is 0).
+  template <bool CLAMP>
   __device__ __forceinline__ void load(const void *, long long, const uint8_t *codes, const uint8_t *exps, uint32_t row, uint32_t rows, int groups,
-                                       int c, int) {
-    const size_t at = min(row, rows - 1);
-    c = min(c, groups * ACT8_GROUP - 8);
-    u = *(const uint2 *)(codes + (at * groups * ACT8_GROUP + c));
-    e = exps[at * groups + c / ACT8_GROUP];
+                                       int c, int n) {
+    if (CLAMP) row = min(row, rows - 1), c = min(c, groups * ACT8_GROUP - 8);
+    else u = make_uint2(0u, 0u), e = 127u;
+    if (CLAMP || n > 0) {
+      const size_t at = (size_t)row * groups;
+      u = *(const uint2 *)(codes + (at * ACT8_GROUP + c));
+      e = exps[at + c / ACT8_GROUP];
+    }
   }
   __device__ __forceinline__ void take(float *v) const {
     act8_decode4(u.x, e, v), act8_decode4(u.y, e, v + 4);
@@ -65,11 +70,11 @@ __device__ __forceinline__ void sums_add(float4 *lds, int slot, const float (&v)
 // A team walks rows team, team + teams, ... of one group of rows (blockIdx.y) that share their gates, or, where there are many
 // groups, whole groups one after another (by_unit); `each` rows have one row of gates.
 // Bound by memory, with 8 waves a compute unit (150 to 220 registers a thread: parameters, sums and two rows): 32 768 x 4 096 bf16 RMS 349 us = 4.6 TB/s
-// exact, 346 (3.9) from codes, with a gate for each element 411 (5.2) and 451 (4.2); LN 362; 65 536 x 1 024 164 (4.9) and 183 (3.7).  Decoding and the
+// exact, 324 (4.2) from codes, with a gate for each element 412 (5.2) and 409 (4.6); LN 362; 65 536 x 1 024 163 (4.9) and 170 (4.0).  Decoding and the
 // products of fp32 rows are what keeps codes and LN from the rate of a copy; 128 registers, and twice the waves, spill: 752 us in place of 349.
 template <int T, bool LAYER, int NCH, int BLOCK, bool WAVES, bool KEEP8>
 __global__ __launch_bounds__(BLOCK, 2) void block_norm_bwd_kernel(BnArgs a) {
-  constexpr bool IN_LDS = BLOCK == 1024 && NCH == 1;
+  constexpr bool IN_LDS = BLOCK == 1024 && NCH == 1, AT_ONCE = KEEP8 && BLOCK == 512;
   __shared__ float team_sums[BLOCK == 512 ? BLOCK * 8 : 1];
   __shared__ float red[64];
   extern __shared__ __attribute__((aligned(16))) float4 bn_sums[];       // IN_LDS: [wanted set, SET_PRE_B apart][2][BLOCK]
@@ -113,7 +118,9 @@ __global__ __launch_bounds__(BLOCK, 2) void block_norm_bwd_kernel(BnArgs a) {
   const uint32_t stride = gridDim.x * teams, first = blockIdx.x * teams + team;
   const uint32_t trips = a.by_unit ? (a.groups + stride - 1) / stride * a.each : (a.each + stride - 1) / stride;
   // The next row's operands are under way while this one is computed: those of y's side from the row's begin on, those of f's side from where
-  // this row's have been taken out of their registers.
+  // this row's have been taken out of their registers.  Codes are so short that both sides can be under way from the row's begin on, AT_ONCE; teams do
+  // without WAVES then, and loads without CLAMP (32 768 x 4 096 bf16 with a gate for each element 409 us; with late loads 449, with clamped ones 453;
+  // exact rows 476, late and with WAVES 413).  With 1 024 threads and half the registers it is the other way round (16 384 x 8 192 723 and 606 us).
   uint32_t unit = a.by_unit ? first : blockIdx.y, in_unit = a.by_unit ? 0 : first;
   Act8Raw<T> raw_gh[NCH], raw_gy[NCH], raw_g[NCH];
   Waiting<T, KEEP8> raw_y[NCH], raw_f[NCH];
@@ -132,7 +139,7 @@ __global__ __launch_bounds__(BLOCK, 2) void block_norm_bwd_kernel(BnArgs a) {
       const int c = 8 * (tx + n * a.T), left = live ? a.C - c : 0;
       if (has_h) {
         raw_gh[n] = act8_load_raw<T>(a.gh, (size_t)row * a.ldgh + c, left);
-        raw_y[n].load(a.y_in, a.ldx, a.y_codes, a.y_exps, row, a.rows, groups8, c, left);
+        raw_y[n].template load<!AT_ONCE>(a.y_in, a.ldx, a.y_codes, a.y_exps, row, a.rows, groups8, c, left);
       }
       if (a.gy) raw_gy[n] = act8_load_raw<T>(a.gy, (size_t)row * a.ldgy + c, left);
     }
@@ -149,7 +156,7 @@ __global__ __launch_bounds__(BLOCK, 2) void block_norm_bwd_kernel(BnArgs a) {
 #pragma unroll
     for (int n = 0; n < NCH; ++n) {
       const int c = 8 * (tx + n * a.T), left = live ? a.C - c : 0;
-      raw_f[n].load(a.f, a.ldf, a.f_codes, a.f_exps, row, a.rows, groups8, c, left);
+      raw_f[n].template load<!AT_ONCE>(a.f, a.ldf, a.f_codes, a.f_exps, row, a.rows, groups8, c, left);
       if (a.gate) raw_g[n] = act8_load_raw<T>(a.gate, (size_t)unit * a.ldg + c, left);
     }
   };
@@ -176,7 +183,20 @@ __global__ __launch_bounds__(BLOCK, 2) void block_norm_bwd_kernel(BnArgs a) {
         raw_y[n].take(hat[n]);
       }
     }
-    if (i + 1 < trips) fetch_y();
+    Waiting<T, KEEP8> now_f[NCH];                // (AT_ONCE)
+    Act8Raw<T> now_g[NCH];
+    float now_f_mean = next_f_mean, now_f_rstd = next_f_rstd;
+    if (AT_ONCE && has_f) {
+#pragma unroll
+      for (int n = 0; n < NCH; ++n) {
+        now_f[n] = raw_f[n];
+        if (a.gate) now_g[n] = raw_g[n];
+      }
+    }
+    if (i + 1 < trips) {
+      fetch_y();
+      if (AT_ONCE && has_f) fetch_f();
+    }
     // (channels behind the width, and rows of a team without one: gradients are 0 there, and what multiplies them is finite)
     if (has_h) {
       float s[2] = {0.f, 0.f};
@@ -224,13 +244,14 @@ __global__ __launch_bounds__(BLOCK, 2) void block_norm_bwd_kernel(BnArgs a) {
     }
     if (has_f) {
       float v[NCH][8], g[NCH][8], s[2] = {0.f, 0.f};
-      const float f_mean = next_f_mean, f_rstd = next_f_rstd;
+      const float f_mean = AT_ONCE ? now_f_mean : next_f_mean, f_rstd = AT_ONCE ? now_f_rstd : next_f_rstd;
 #pragma unroll
       for (int n = 0; n < NCH; ++n) {
-        raw_f[n].take(hat[n]);
-        if (a.gate) act8_unraw<T>(raw_g[n], g[n]);
+        if constexpr (AT_ONCE) now_f[n].take(hat[n]);
+        else raw_f[n].take(hat[n]);
+        if (a.gate) act8_unraw<T>(AT_ONCE ? now_g[n] : raw_g[n], g[n]);
       }
-      if (i + 1 < trips) fetch_f();
+      if (!AT_ONCE && i + 1 < trips) fetch_f();
 #pragma unroll
       for (int n = 0; n < NCH; ++n) {
         const int c = 8 * (tx + n * a.T);
@@ -372,7 +393,7 @@ __global__ __launch_bounds__(BLOCK, 2) void block_norm_bwd_kernel(BnArgs a) {
 
 template <int T, bool LAYER, int NCH, int BLOCK, bool WAVES>
 int launch_bwd(const BnArgs &a, const BnGrid &g, hipStream_t st) {
-  auto k = a.f_codes || a.y_codes ? block_norm_bwd_kernel<T, LAYER, NCH, BLOCK, WAVES, true> : block_norm_bwd_kernel<T, LAYER, NCH, BLOCK, WAVES, false>;
+  auto k = a.f_codes || a.y_codes ? block_norm_bwd_kernel<T, LAYER, NCH, BLOCK, WAVES && BLOCK != 512, true> : block_norm_bwd_kernel<T, LAYER, NCH, BLOCK, WAVES, false>;
   const int in_lds = a.sets & ~(1 << SET_PRE_B), slots = in_lds || !a.sets ? __builtin_popcount(in_lds) : 1;
   const int lds = BLOCK == 1024 && NCH == 1 ? slots * 2 * BLOCK * (int)sizeof(float4) : 0;
   if (lds > 65536 - 1024) DM_HIP(hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
