@@ -247,3 +247,10 @@ def test_relu_gradient_where_an_output_underflows_or_is_nan(dev):
             want = (~(y.detach() <= 0)).double().sum(0)
             assert torch.equal(gb.double(), want), (dtype, split, gb, want, y)
             assert bool(y[:, 5].isnan().all()) and float(gb[5]) == 3 and float(gb[1]) <= 1 and float(gb[4]) == 3
+
+
+def test_an_infinity_in_float32_is_nan_behind_a_relu_too(dev):
+    x, w, b, _ = _case(40, 64, 32, torch.float32, dev, True, False)
+    x[4, 6], x[5, 7] = float('inf'), -float('inf')
+    y = act8.linear(x, w, b, relu=True)
+    assert bool(y[4:6].isnan().all()) and bool(y[:4].isfinite().all()) and bool(y[6:].isfinite().all())
