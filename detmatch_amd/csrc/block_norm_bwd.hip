@@ -11,7 +11,7 @@ template <int T, bool KEEP8>
 struct Waiting {
   Act8Raw<T> r;
   template <bool>
-  __device__ __forceinline__ void load(const void *p, long long ld, const uint8_t *, const uint8_t *, uint32_t row, uint32_t, int, int c, int n) {
+  __device__ __forceinline__ void load(const void *p, long long ld, const uint8_t *, const uint8_t *, uint32_t row, int, int c, int n) {
     r = act8_load_raw<T>(p, (size_t)row * ld + c, n);
   }
   __device__ __forceinline__ void take(float *v) const { act8_unraw<T>(r, v); }
@@ -21,11 +21,12 @@ template <int T>
 struct Waiting<T, true> {
   uint2 u;
   uint32_t e;
-  // Behind a row's end and for a team without a row: zeros, or, CLAMP, other codes (what they are multiplied with is 0).
+  // Behind a row's end and for a team without a row: zeros.  CLAMP: behind a row's end other codes of the same row, without a branch.  (Gradients are 0 there; should
+  // a code be a nan, that row's sums are nan already.  Another row's codes would not do: 0 * nan is nan.  So CLAMP is for teams that never lack a row.)
   template <bool CLAMP>
-  __device__ __forceinline__ void load(const void *, long long, const uint8_t *codes, const uint8_t *exps, uint32_t row, uint32_t rows, int groups,
+  __device__ __forceinline__ void load(const void *, long long, const uint8_t *codes, const uint8_t *exps, uint32_t row, int groups,
                                        int c, int n) {
-    if (CLAMP) row = min(row, rows - 1), c = min(c, groups * ACT8_GROUP - 8);
+    if (CLAMP) c = min(c, groups * ACT8_GROUP - 8);
     else u = make_uint2(0u, 0u), e = 127u;
     if (CLAMP || n > 0) {
       const size_t at = (size_t)row * groups;
@@ -116,7 +117,10 @@ __global__ __launch_bounds__(BLOCK, 2) void block_norm_bwd_kernel(BnArgs a) {
     }
   };
   const uint32_t stride = gridDim.x * teams, first = blockIdx.x * teams + team;
-  const uint32_t trips = a.by_unit ? (a.groups + stride - 1) / stride * a.each : (a.each + stride - 1) / stride;
+  // Teams of a workgroup meet in the sums: all make as many trips as the first, the last ones perhaps without a row of their own.  Where codes are clamped a
+  // workgroup is one team (1 024 threads), and walks its own rows alone (there are at most as many workgroups as rows or groups).
+  const uint32_t ahead = KEEP8 && !AT_ONCE ? first : 0;
+  const uint32_t trips = a.by_unit ? (a.groups - ahead + stride - 1) / stride * a.each : (a.each - ahead + stride - 1) / stride;
   // The next row's operands are under way while this one is computed: those of y's side from the row's begin on, those of f's side from where
   // this row's have been taken out of their registers.  Codes are so short that both sides can be under way from the row's begin on, AT_ONCE; teams do
   // without WAVES then, and loads without CLAMP (32 768 x 4 096 bf16 with a gate for each element 409 us; with late loads 449, with clamped ones 453;
@@ -139,7 +143,7 @@ __global__ __launch_bounds__(BLOCK, 2) void block_norm_bwd_kernel(BnArgs a) {
       const int c = 8 * (tx + n * a.T), left = live ? a.C - c : 0;
       if (has_h) {
         raw_gh[n] = act8_load_raw<T>(a.gh, (size_t)row * a.ldgh + c, left);
-        raw_y[n].template load<!AT_ONCE>(a.y_in, a.ldx, a.y_codes, a.y_exps, row, a.rows, groups8, c, left);
+        raw_y[n].template load<!AT_ONCE>(a.y_in, a.ldx, a.y_codes, a.y_exps, row, groups8, c, left);
       }
       if (a.gy) raw_gy[n] = act8_load_raw<T>(a.gy, (size_t)row * a.ldgy + c, left);
     }
@@ -156,7 +160,7 @@ __global__ __launch_bounds__(BLOCK, 2) void block_norm_bwd_kernel(BnArgs a) {
 #pragma unroll
     for (int n = 0; n < NCH; ++n) {
       const int c = 8 * (tx + n * a.T), left = live ? a.C - c : 0;
-      raw_f[n].template load<!AT_ONCE>(a.f, a.ldf, a.f_codes, a.f_exps, row, a.rows, groups8, c, left);
+      raw_f[n].template load<!AT_ONCE>(a.f, a.ldf, a.f_codes, a.f_exps, row, groups8, c, left);
       if (a.gate) raw_g[n] = act8_load_raw<T>(a.gate, (size_t)unit * a.ldg + c, left);
     }
   };
