@@ -13,7 +13,7 @@ off by at most 2^-4 of a value (half a step), or 2^-10 of the group's scale belo
 `pack` / `unpack` are plain functions (no gradient).  The forward pass and the input gradient of `linear` see x and w as they are;
 only the weight gradient sees unpack(pack(x))."""
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -77,6 +77,27 @@ def _device_of(*tensors):
     return dev
 
 
+def _refuse_trace():
+    """Kernels called outside of an autograd function leave no trace: torch.jit.trace would record empty buffers in their place."""
+    if torch._C._get_tracing_state() is not None:
+        raise NotImplementedError('torch.jit.trace cannot record these operators where no input needs a gradient')
+
+
+def _wants_grad(*tensors):
+    """Does the call go through the autograd function?  Where it does not, what the function refuses by itself is refused here: forward-mode
+    derivatives, which would be lost, and traces."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError('these operators have no forward-mode derivatives')
+    _refuse_trace()
+    return False
+
+
 def _dtype_code(t, what):
     code = DTYPES.get(t.dtype)
     if code is None:
@@ -104,6 +125,7 @@ def pack(x):
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError('pack needs at least one channel, got shape %s' % (tuple(x.shape),))
     code = _dtype_code(x, 'x')
+    _refuse_trace()
     dev = _device_of(x)
     with _on(dev):
         r = rows_view(x.detach() if x.requires_grad else x)
@@ -121,6 +143,7 @@ def unpack(kept, dtype=None):
     value."""
     if not isinstance(kept, Act8):
         raise TypeError('unpack takes what pack returned, got %s' % type(kept).__name__)
+    _refuse_trace()
     width = kept.shape[-1]
     rows, groups = kept.shape.numel() // width, (width + GROUP - 1) // GROUP
     for t, shape, name in ((kept.codes, (rows, groups * GROUP), 'codes'), (kept.exps, (rows, groups), 'exps')):
@@ -254,7 +277,7 @@ def linear(x, w, b=None, relu=False):
     Kept for the backward pass: pack(x) where w needs a gradient, one bit per output where there is a ReLU, w where x needs a
     gradient.  gw = g^T unpack(pack(x)), gx = g w, gb = sum of g over rows, g = the gradient behind the ReLU (0 where its output,
     as it is stored, is 0).  float32 operands are multiplied in pieces: a result in which an infinity takes part is nan.
-    x may be overwritten after the call.  Differentiable once."""
+    x may be overwritten after the call.  Differentiable once, in reverse mode; a forward-mode derivative is refused."""
     if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1]:
         raise ValueError('x (..., in) and w (out, in) are wanted, got %s and %s' % (tuple(x.shape), tuple(w.shape)))
     if b is not None and tuple(b.shape) != (w.shape[0],):
@@ -265,11 +288,12 @@ def linear(x, w, b=None, relu=False):
     for t, name in ((w, 'w'), (b, 'b')):
         if t is not None and t.dtype != x.dtype:
             raise TypeError('%s is %s, x is %s: one type is wanted' % (name, t.dtype, x.dtype))
+    grad = _wants_grad(x, w, b)
     _device_of(x, w, b)
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     if max(x2.shape[0], w.shape[0], w.shape[1]) > _MAX:
         raise ValueError('sizes up to %d are wanted, got x %s, w %s' % (_MAX, tuple(x.shape), tuple(w.shape)))
-    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or (b is not None and b.requires_grad)):
+    if grad:
         y = _Linear8.apply(x2, w, b, bool(relu))
     else:
         m, k = x2.shape

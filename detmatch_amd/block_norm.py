@@ -15,7 +15,7 @@ from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .act8 import DTYPES, GROUP, _MAX, _device_of, _dtype_code, _on, row_stride, rows_view
+from .act8 import DTYPES, GROUP, _MAX, _device_of, _dtype_code, _on, _wants_grad, row_stride, rows_view
 
 KINDS = {'rms': 0, 'layer': 1}
 GATE_ACTS = {None: 0, 'none': 0, 'sigmoid': 1, 'tanh': 2}
@@ -159,11 +159,9 @@ class _ResidualNorm(Function):
         return (dx, df, *out, None, None, None)
 
 
-def _apply(x, f, gate, scale, post_w, post_b, pre_w, pre_b, meta, pre, keep8):
-    if torch.is_grad_enabled():
-        for t in (x, f, gate, scale, post_w, post_b, pre_w, pre_b):
-            if t is not None and t.requires_grad:
-                return _ResidualNorm.apply(x, f, gate, scale, post_w, post_b, pre_w, pre_b, meta, pre, keep8)
+def _apply(grad, x, f, gate, scale, post_w, post_b, pre_w, pre_b, meta, pre, keep8):
+    if grad:
+        return _ResidualNorm.apply(x, f, gate, scale, post_w, post_b, pre_w, pre_b, meta, pre, keep8)
     with _on(x.device):
         return _forward(x, f, gate, scale, post_w, post_b, pre_w, pre_b, meta, pre, None, None)
 
@@ -172,7 +170,7 @@ _WIDTH = []
 
 
 def _check(x, f, gate, scale, post_w, post_b, pre_w, pre_b, kind, eps, gate_act, post):
-    """What both entry points refuse; -> (rows, width)"""
+    """What both entry points refuse; -> (rows, width, does the call go through the autograd function)"""
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError('x (..., channels) is wanted, got %s' % (tuple(x.shape),))
     dtype = x.dtype
@@ -218,12 +216,13 @@ def _check(x, f, gate, scale, post_w, post_b, pre_w, pre_b, kind, eps, gate_act,
             raise ValueError('scale has %d elements: a number, or a tensor of one' % scale.numel())
         if scale.dtype != dtype and scale.dtype != torch.float32:
             raise TypeError('scale is %s: float32 or %s' % (scale.dtype, dtype))
+    grad = _wants_grad(x, f, gate, scale, post_w, post_b, pre_w, pre_b)
     _device_of(x, f, gate, scale, post_w, post_b, pre_w, pre_b)
     if not _WIDTH:
         _WIDTH.append(max_width())
     if width > _WIDTH[0]:
         raise ValueError('%d channels: up to %d' % (width, _WIDTH[0]))
-    return rows, width
+    return rows, width, grad
 
 
 def residual_norm(x, f, scale=1.0, gate=None, gate_act=None, post=True, post_w=None, post_b=None, pre=True, pre_w=None, pre_b=None,
@@ -237,15 +236,15 @@ def residual_norm(x, f, scale=1.0, gate=None, gate_act=None, post=True, post_w=N
     scale: a number, or a tensor of one element (with a gradient).  gate: (C,) for all rows; (G, C) (any leading shape): each for
     rows / G consecutive rows, a sample's or (G = rows) a row's own; gate_act None, 'sigmoid' or 'tanh' of it.  Weights (C,) in x's type or
     float32; None: 1.  Biases with kind = 'layer' only.  Statistics and sums are fp32; h is the norm of y before y is rounded.
-    keep8: keep f and y in 8 bits for the backward pass.  Differentiable once."""
+    keep8: keep f and y in 8 bits for the backward pass.  Differentiable once, in reverse mode; a forward-mode derivative is refused."""
     if f is None:
         raise ValueError('f is None: norm_rows is the norm alone')
     if not pre and (pre_w is not None or pre_b is not None):
         raise ValueError('pre_w / pre_b without pre')
     tensor, number = (scale, 0.0) if isinstance(scale, torch.Tensor) else (None, float(scale))
-    rows, width = _check(x, f, gate, tensor, post_w, post_b, pre_w, pre_b, kind, eps, gate_act, post)
+    rows, width, grad = _check(x, f, gate, tensor, post_w, post_b, pre_w, pre_b, kind, eps, gate_act, post)
     flat = x.dim() == 2
-    y, h = _apply(x if flat else x.reshape(rows, width), f if flat else f.reshape(rows, width),
+    y, h = _apply(grad, x if flat else x.reshape(rows, width), f if flat else f.reshape(rows, width),
                   gate if gate is None or gate.dim() == 2 else gate.reshape(-1, width), tensor, post_w, post_b, pre_w, pre_b,
                   (bool(post), KINDS[kind], GATE_ACTS[gate_act], float(eps), number), bool(pre), bool(keep8))
     return (y, h) if flat else (y.view(x.shape), None if h is None else h.view(x.shape))
@@ -253,8 +252,8 @@ def residual_norm(x, f, scale=1.0, gate=None, gate_act=None, post=True, post_w=N
 
 def norm_rows(x, w=None, b=None, kind='rms', eps=1e-6, keep8=False):
     """N(x) * w + b over the last dimension of x (float32, bfloat16, float16); w, b (C,) in x's type or float32, or None."""
-    rows, width = _check(x, None, None, None, None, None, w, b, kind, eps, None, True)
+    rows, width, grad = _check(x, None, None, None, None, None, w, b, kind, eps, None, True)
     flat = x.dim() == 2
-    _, h = _apply(x if flat else x.reshape(rows, width), None, None, None, None, None, w, b, (False, KINDS[kind], 0, float(eps), 1.0), True,
+    _, h = _apply(grad, x if flat else x.reshape(rows, width), None, None, None, None, None, w, b, (False, KINDS[kind], 0, float(eps), 1.0), True,
                   bool(keep8))
     return h if flat else h.view(x.shape)
