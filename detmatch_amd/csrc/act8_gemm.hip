@@ -800,6 +800,8 @@ typedef Shape<2, 4, 4, 2, 64, 2, 1> BigForward;
 typedef Shape<2, 2, 4, 2, 32, 3, 1> BigWeight;
 
 constexpr long long A8_MAX_PITCH = (1ll << 31) / 512 - 8;
+// sizes are 32-bit numbers in the kernels, which add a tile's width to them
+constexpr int A8_MAX_SIZE = 0x7fffffff - 1023;
 
 struct Plan {
   int big, bm, bn, bk, tiles_m, tiles_n, splits, steps_per_split;
@@ -882,7 +884,7 @@ static bool a8_regs(int form, int dtype, const void *A, long long lda, const voi
 
 extern "C" size_t dm_act8_gemm_workspace_bytes(int form, int dtype, const void *A, long long lda, const void *B, long long ldb, int padded, int M,
                                                int N, int K) {
-  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  if (M <= 0 || N <= 0 || K <= 0 || M > A8_MAX_SIZE || N > A8_MAX_SIZE || K > A8_MAX_SIZE) return 0;
   const Plan p = a8_plan(form, dtype, a8_regs(form, dtype, A, lda, B, ldb, padded, M, N, K), M, N, K);
   return p.splits > 1 ? dm_align(((size_t)p.splits * M * N + (form == 2 ? (size_t)p.splits * M : 0)) * sizeof(float)) : 0;
 }
@@ -893,6 +895,7 @@ extern "C" int dm_act8_gemm(int form, int dtype, const void *A, long long lda, c
   hipStream_t st = (hipStream_t)stream;
   if (form < 0 || form > 2 || dtype < ACT8_F32 || dtype > ACT8_F16 || M <= 0 || N <= 0 || K <= 0 || !A || !B || !C)
     return DM_ERR_INVALID_ARG;
+  if (M > A8_MAX_SIZE || N > A8_MAX_SIZE || K > A8_MAX_SIZE) return DM_ERR_INVALID_ARG;
   if ((form == 2) != (exps != nullptr) || (form != 2 && rowsum) || (form == 2 && (bias || relu || sign_bits))) return DM_ERR_INVALID_ARG;
   if (lda < (form == 2 ? M : K) || ldb < (form == 0 ? K : N)) return DM_ERR_INVALID_ARG;
   if (form == 2 && (ldb % 32 || ((uintptr_t)B & 15))) return DM_ERR_INVALID_ARG;
@@ -920,7 +923,7 @@ extern "C" int dm_act8_gemm(int form, int dtype, const void *A, long long lda, c
 
 extern "C" int dm_act8_mask_rows(const void *x, int dtype, long long rows, int width, long long ld, const uint32_t *sign_bits, void *out,
                                  int ldo, dm_stream_t stream) {
-  if (dtype < ACT8_F32 || dtype > ACT8_F16 || rows < 0 || width <= 0 || ld < width || ldo < width || ldo % 8) return DM_ERR_INVALID_ARG;
+  if (dtype < ACT8_F32 || dtype > ACT8_F16 || rows < 0 || width <= 0 || ld < width || ldo < width || ldo % 8 || ldo > A8_MAX_SIZE) return DM_ERR_INVALID_ARG;
   if (rows == 0) return DM_OK;
   if (!x || !out || ((uintptr_t)out & 15)) return DM_ERR_INVALID_ARG;
   const long long blocks = (rows * (ldo / 8) + 255) / 256;

@@ -1112,7 +1112,7 @@ int dm_act8_unpack(const uint8_t *codes, const uint8_t *exps, long long rows, in
  *   form 1  C[M][N] = A[M][K] . B[K][N]
  *   form 2  C[M][N] = A[K][M]^T . deq(B)[K][N]                 B codes, row pitch ldb = 32 * groups, exps (K, groups) as
  *                                                              dm_act8_pack writes them; rowsum (M) or NULL: sums of A's columns
- * Rows of A and B have pitches lda, ldb; C is dense.  16-bit operands at any address; those whose addresses are multiples of 16 bytes, whose pitches
+ * M, N, K <= 2^31 - 1024 (ldo too).  Rows of A and B have pitches lda, ldb; C is dense.  16-bit operands at any address; those whose addresses are multiples of 16 bytes, whose pitches
  * are multiples of 8 elements (<= 4 194 296) and whose rows are whole multiples of 8 elements go straight into LDS.  padded, bit 0 for A, bit 1 for B: the rows may
  * be read up to the next multiple of 8 elements, and are 0 there where they run along the contraction (dm_act8_mask_rows without bits
  * makes such a copy).  Few output tiles: the contraction is split and the parts (workspace, dm_act8_gemm_workspace_bytes of the same arguments)
