@@ -276,7 +276,8 @@ def linear(x, w, b=None, relu=False):
 
     Kept for the backward pass: pack(x) where w needs a gradient, one bit per output where there is a ReLU, w where x needs a
     gradient.  gw = g^T unpack(pack(x)), gx = g w, gb = sum of g over rows, g = the gradient behind the ReLU (0 where its output,
-    as it is stored, is 0).  float32 operands are multiplied in pieces: a result in which an infinity takes part is nan.
+    as it is stored, is 0).  float32 operands are multiplied in pieces: a result in which an infinity takes part is nan, and less than
+    2^-133 is lost of a value below 2^-109.
     x may be overwritten after the call.  Differentiable once, in reverse mode; a forward-mode derivative is refused."""
     if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1]:
         raise ValueError('x (..., in) and w (out, in) are wanted, got %s and %s' % (tuple(x.shape), tuple(w.shape)))

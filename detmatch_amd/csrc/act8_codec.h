@@ -2,7 +2,8 @@
 //
 //   amax = max |x| over the finite values of the group;  e = the least exponent with amax <= 448 * 2^e (448 = 1.75 * 2^8 is the
 //   largest e4m3 value), at least -127; e = 0 for a group of zeros;  code = e4m3(x * 2^-e), round to nearest even.
-// The scale is a power of two, so the product is exact and a code's value, 4 significant bits times 2^e, is exact in bf16 and fp32.
+// The scale is a power of two, so the product is exact and a code's value, 4 significant bits times 2^e, is exact in fp32; in bf16 too where it is a multiple
+// of 2^-133, bf16's least number: every code from e = -124 on, and every code of a row that was bf16 or fp16.
 // Values that would round to 2^128 (e = 120, code 256) stay at 240 * 2^120; inf and nan become nan (e4m3 has no inf).
 #pragma once
 #include "dm_common.h"

@@ -2,9 +2,10 @@
 //   form 0   C[M][N] = A[M][K] . B[N][K]^T (+ bias, ReLU, sign bits)   forward            y  = x w^T + b
 //   form 1   C[M][N] = A[M][K] . B[K][N]                               input gradient     gx = gy w
 //   form 2   C[M][N] = A[K][M]^T . deq(B)[K][N] (+ row sums)           weight gradient    gw = gy^T x8, gb = sum of gy
-// All on the 16-bit matrix instructions (v_mfma_f32_32x32x16), accumulated in fp32.  deq(code) is exact in bf16, so form 2 loses nothing
-// there.  fp32 operands are cut into three bf16 pieces (8 + 8 + 8 bits: exact for finite values) while they are staged; a product
-// of two such operands takes the 6 of the 9 piece products that matter in fp32, a product with codes takes 3.
+// All on the 16-bit matrix instructions (v_mfma_f32_32x32x16, subnormal numbers included), accumulated in fp32.  deq(code) is exact in bf16, so form 2 loses
+// nothing there.  fp32 operands are cut into three bf16 pieces (8 + 8 + 8 bits) while they are staged; a product of two such operands takes the 6 of the 9 piece
+// products that matter in fp32, a product with codes takes 3.  The pieces are all of a finite value from 2^-109 on; below that, and of a code of an fp32 row, what
+// lies under 2^-133, bf16's least number, is lost.
 //
 // A wave owns FM x FN blocks of 32 x 32; the matrix instruction gets its operands swapped (rows of its result = columns of C), so that a
 // lane ends with 4 neighbouring elements of a row of C.  Few output tiles and a long contraction: the contraction is split over
