@@ -234,8 +234,8 @@ def residual_norm(x, f, scale=1.0, gate=None, gate_act=None, post=True, post_w=N
         h = N(y) * pre_w + pre_b    (pre = False: h is None)
 
     scale: a number, or a tensor of one element (with a gradient).  gate: (C,) for all rows; (G, C) (any leading shape): each for
-    rows / G consecutive rows, a sample's or (G = rows) a row's own; gate_act None, 'sigmoid' or 'tanh' of it.  Weights (C,) in x's type or
-    float32; None: 1.  Biases with kind = 'layer' only.  Statistics and sums are fp32; h is the norm of y before y is rounded.
+    rows / G consecutive rows, a sample's or (G = rows) a row's own; gate_act None, 'sigmoid' or 'tanh' of it.  (The backward pass is slow for G > 64
+    groups of hundreds of rows: it walks each one after the other.)  Weights (C,) in x's type or float32; None: 1.  Biases with kind = 'layer' only.  Statistics and sums are fp32; h is the norm of y before y is rounded.
     keep8: keep f and y in 8 bits for the backward pass.  Differentiable once, in reverse mode; a forward-mode derivative is refused."""
     if f is None:
         raise ValueError('f is None: norm_rows is the norm alone')

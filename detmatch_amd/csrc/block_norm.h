@@ -121,7 +121,9 @@ inline bool bn_plan(int C, bool backward, BnPlan *p) {
   return p->nch <= 2;
 }
 
-// workgroups of the backward kernel: x for one group, y groups (by_unit: all groups in x)
+// Workgroups of the backward kernel: x for one group, y groups (by_unit: all groups in x).  From 65 groups on a team takes whole groups, so that a group's gate
+// gradient is complete in its registers.  That suits short groups: a row each, or a few rows.  Long ones leave most of the chip idle, as there are no more teams at
+// work than groups: 64 groups of 1 000 x 256 bf16 52 us, 65 groups 2 792.
 struct BnGrid {
   int x, y, by_unit;
 };

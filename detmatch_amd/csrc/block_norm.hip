@@ -62,7 +62,7 @@ __device__ __forceinline__ void row_stats(const BnArgs &a, const float (&v)[NCH]
 
 // A workgroup's teams walk the rows with the grid's stride.  The next row's operands are under way while this one is computed.
 // Bound by memory: 32 768 x 4 096 bf16 RMS 212 us = 5.0 TB/s, with a gate for each element 243 (5.5), and keeping codes 292 (5.5); LN 250; 16 384 x 640
-// fp32 LN 42 (4.0), with the gates of a sample 49; 8 192 x 2 048 keeping codes 38 (4.4).
+// fp32 LN 42 (4.0), with the gates of a sample 49 (3.4: gates that rows share are loaded and activated for each row); 8 192 x 2 048 keeping codes 38 (4.4).
 template <int T, bool LAYER, int NCH, int BLOCK, bool WAVES>
 __global__ __launch_bounds__(BLOCK, NCH == 1 ? 4 : 2) void block_norm_fwd_kernel(BnArgs a) {
   __shared__ float red[64];

@@ -51,7 +51,7 @@ __device__ __forceinline__ uint32_t in_vector(uint32_t v) {
 }
 
 // Sums over the rows that a thread walks, 8 channels of one set, stay in registers; with 1 024 threads to a row there are too few of those, and the
-// sums lie in LDS (16 384 x 8 192 bf16: 607 us against 902 with registers that spill; at 4 096 channels LDS costs 595 us against 343).
+// sums lie in LDS (16 384 x 8 192 bf16, exact RMS rows: 514 us against 620 with registers that spill, from codes 532 and 670; at 4 096 channels LDS costs 595 us against 343).
 template <int BLOCK>
 __device__ __forceinline__ float4 *sums_at(float4 *lds, int slot, int half) {
   return lds + (slot * 2 + half) * BLOCK + threadIdx.x;
@@ -73,6 +73,9 @@ __device__ __forceinline__ void sums_add(float4 *lds, int slot, const float (&v)
 // Bound by memory, with 8 waves a compute unit (150 to 220 registers a thread: parameters, sums and two rows): 32 768 x 4 096 bf16 RMS 349 us = 4.6 TB/s
 // exact, 324 (4.2) from codes, with a gate for each element 412 (5.2) and 409 (4.6); LN 362; 65 536 x 1 024 163 (4.9) and 170 (4.0).  Decoding and the
 // products of fp32 rows are what keeps codes and LN from the rate of a copy; 128 registers, and twice the waves, spill: 752 us in place of 349.
+// Above 4 096 channels 1 024 threads have 128 registers each, and rows come one at a time: 16 384 x 8 192 bf16 RMS 507 us = 3.2 TB/s exact, 528 (2.6) from codes, with
+// a gate for each element 673 (2.8); LN 778 (2.1) and 789 (1.7).  Above 8 192 channels a thread has twice 8 channels and the sums spill: 8 192 x 16 384 RMS 1 619 us = 1.0
+// TB/s, LN from codes 3 030 (0.45): right, but far from fast.
 template <int T, bool LAYER, int NCH, int BLOCK, bool WAVES, bool KEEP8>
 __global__ __launch_bounds__(BLOCK, 2) void block_norm_bwd_kernel(BnArgs a) {
   constexpr bool IN_LDS = BLOCK == 1024 && NCH == 1, AT_ONCE = KEEP8 && BLOCK == 512;
@@ -124,7 +127,7 @@ __global__ __launch_bounds__(BLOCK, 2) void block_norm_bwd_kernel(BnArgs a) {
   // The next row's operands are under way while this one is computed: those of y's side from the row's begin on, those of f's side from where
   // this row's have been taken out of their registers.  Codes are so short that both sides can be under way from the row's begin on, AT_ONCE; teams do
   // without WAVES then, and loads without CLAMP (32 768 x 4 096 bf16 with a gate for each element 409 us; with late loads 449, with clamped ones 453;
-  // exact rows 476, late and with WAVES 413).  With 1 024 threads and half the registers it is the other way round (16 384 x 8 192 723 and 606 us).
+  // exact rows 476, late and with WAVES 413).  With 1 024 threads and half the registers it is the other way round (16 384 x 8 192 with a gate for each element 969 and 688 us).
   uint32_t unit = a.by_unit ? first : blockIdx.y, in_unit = a.by_unit ? 0 : first;
   Act8Raw<T> raw_gh[NCH], raw_gy[NCH], raw_g[NCH];
   Waiting<T, KEEP8> raw_y[NCH], raw_f[NCH];

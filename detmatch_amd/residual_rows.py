@@ -3,9 +3,11 @@
     stream, h = x, N(x; norm[0])
     for each block i:  f = fc2(relu(fc1(h)));  stream, h = stream + scale * act(gate) * N(f; post),  N(that; norm[i + 1])
 
-The last h is the result.  A block is five launches: the two layers are act8.linear, everything between them and the next block's first
-layer is one pass of block_norm.residual_norm.  Unlike BatchNorm, no statistics are shared between rows: a row's result does not depend on
-which rows, labelled or unlabelled, are in its batch, nor on training or evaluation mode."""
+The last h is the result.  The two layers are act8.linear, everything between them and the next block's first layer is one pass of
+block_norm.residual_norm: a block's forward pass is 3 launches at inference and 5 in training (each layer packs its input), and one more for
+each layer whose contraction is split or whose rows are copied.  Unlike BatchNorm, no statistics are shared between rows: a row's result
+does not depend on which rows, labelled or unlabelled, are in its batch (their number may choose another split of a product, and with
+it another rounding), nor on training or evaluation mode."""
 import torch
 from torch import nn
 
